@@ -1748,9 +1748,11 @@ void decode_update(const Tensor& tok, Tensor out_tokens, const optional<Tensor>&
 }  // namespace
 
 void bind_layered(py::module_& m);  // csrc/host/bind_layered.cpp
+void bind_drafts(py::module_& m);   // csrc/host/bind_drafts.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_layered(m);
+  bind_drafts(m);
   m.doc() = "gfx950 (MI355X) HIP kernels + native host runtime";
   m.def("decode_ws_dirty_tickets", &decode_ws_dirty_tickets, "per decode workspace: tickets not at zero");
   m.def("gemm", &gemm, "bf16 MFMA GEMM C = act(rstd(A) A W^T + U UB^T + bias) + R", py::arg("a"), py::arg("w"),

@@ -473,6 +473,28 @@ class CausalLM(nn.Module):
             x, residual = layer.mlp(o, residual, defer)
         return self.final_norm(x, residual)
 
+    @torch.no_grad()
+    def verify(self, tokens, tree, kv_len, kv_start, cache):
+        """One forward over drafted tokens [B, N] (``ops.draft_tree`` with pos0 = kv_len - kv_start): every node of a row is a row of its own that
+        sees the row's cache and its ancestors. Returns (final hidden [B*N, H], the layers' rotated [q | k | v] rows, from which
+        ``ops.tree_accept`` appends the accepted nodes to the cache). bf16 / fp32 caches."""
+        cfg = self.cfg
+        if getattr(cache, "fp8", False):
+            raise ValueError("drafted tokens are checked over a bf16 or fp32 cache")
+        cos, sin = self.rope(tokens.device)
+        pos = tree.pos.reshape(-1)
+        x = self.embed_tokens(tokens.reshape(-1), pos)
+        residual, drafts = None, []
+        for li, layer in enumerate(self.layers):
+            qkv, residual, rotated = layer.attn_in_rope(x, residual, (pos, cos, sin) if cos is not None else None)
+            if cos is not None and not rotated:
+                qkv = ops.rope_qkv(qkv, pos, cos, sin, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim)
+            drafts.append(qkv)
+            o = ops.tree_attention(qkv, cache.k[li], cache.v[li], kv_len, tree, cfg.num_heads, kv_start, cfg.sliding_window)
+            x, residual = layer.mlp(o, residual)
+        return self.final_norm(x, residual), drafts
+
+
     # ------------------------------------------------------------------ LoRA
     def add_lora(self, r: int = 16, alpha: float = 32.0, targets=None, dropout: float = 0.0, seed: int = 0):
         """Attach PEFT-style LoRA adapters (A kaiming-uniform, B zero) to the target projections."""

@@ -1,0 +1,106 @@
+"""Checking drafted tokens: a forward over a tree of guesses per row instead of one token (no grad).
+
+A step of it: :func:`draft_tree` makes the plan of the batch's trees (node 0 of a row is its last token, every other node continues an earlier
+one); the model runs all nodes as rows, at the positions ``tree.pos``, its layers attending with :func:`tree_attention` over the cache and the
+node's own ancestors (``CausalLM.verify``); what the model would write after each node is sampled from the logits; :func:`tree_accept` follows it
+through the tree and appends the keys and values of the nodes on that path to the cache of every layer. Nodes that were not
+accepted never touch the cache. All of it stays on the device and can be captured in a graph."""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import List, Optional
+
+import torch
+
+from . import reference as ref
+from ._ext import native, on_gpu
+
+MAX_NODES = 64  # a node's ancestors are the bits of one word
+
+
+@dataclass
+class DraftTree:
+    """Trees of a batch, [rows, nodes] each: parent int32 (as given), see int64 (bit j: the node itself or its ancestor j; 0: not
+    a node), pos int32."""
+
+    parent: torch.Tensor
+    see: torch.Tensor
+    pos: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.see.shape
+
+
+def _ints(t, name, shape, like):
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or t.device != like.device:
+        raise ValueError(f"{name}: int32 {tuple(shape)} on {like.device} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0: Optional[torch.Tensor] = None) -> DraftTree:
+    """The plan of drafted trees: ``parent`` int32 [rows, nodes <= 64] holds an earlier node of the row for each (anything else: none, a tree of its
+    own), ``nodes`` int32 [rows] how many of a row's are nodes (0: the row idles; default all), ``pos0`` int32 [rows] the position
+    of node 0 (default 0)."""
+    if parent.dim() != 2 or not 1 <= parent.shape[1] <= MAX_NODES:
+        raise ValueError(f"parent: [rows, 1 .. {MAX_NODES} nodes] expected, got {tuple(parent.shape)}")
+    parent = _ints(parent, "parent", parent.shape, parent)
+    nodes = None if nodes is None else _ints(nodes, "nodes", parent.shape[:1], parent)
+    pos0 = None if pos0 is None else _ints(pos0, "pos0", parent.shape[:1], parent)
+    see, pos = native().draft_tree(parent, nodes, pos0) if on_gpu(parent) else ref.draft_tree(parent, nodes, pos0)
+    return DraftTree(parent, see, pos)
+
+
+def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, tree: DraftTree, Hq: int,
+                   kv_start: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted tokens -> [rows * nodes, Hq * D]. ``qkv`` [rows * nodes, >= (Hq + 2 Hkv) * D] holds the nodes' rotated rows [q | k | v];
+    node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
+    key; with ``window`` only those less than ``window`` positions before it. Nothing is appended to the caches; rows that are not
+    nodes come out as zeros. What other nodes hold, NaN among it, does not reach a node."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    B, Hkv, Smax, D = k_cache.shape
+    N = tree.shape[1]
+    if tree.shape[0] != B or qkv.dim() != 2 or qkv.shape[0] != B * N:
+        raise ValueError(f"qkv: {B} rows of {N} nodes expected, got {tuple(qkv.shape)} for a tree {tuple(tree.shape)}")
+    if Hkv < 1 or Hq < 1 or Hq % Hkv or qkv.shape[1] < (Hq + 2 * Hkv) * D:
+        raise ValueError(f"{Hq} heads over {Hkv} of {D} do not fit {qkv.shape[1]} columns")
+    if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
+        raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}: an fp8 cache is read by decode_step_attention only")
+    if window < 0:
+        raise ValueError(f"window {window}")
+    kv_len = _ints(kv_len, "kv_len", (B,), qkv)
+    kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if out is None:
+        out = torch.empty(B * N, Hq * D, dtype=qkv.dtype, device=qkv.device)
+    if on_gpu(qkv):
+        native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale)
+    else:
+        out.copy_(ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale))
+    return out
+
+
+def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, drafts: List[torch.Tensor], k_cache: torch.Tensor,
+                v_cache: torch.Tensor, kv_len: torch.Tensor):
+    """The path that the model agrees with -> (its length int32 [rows], its nodes int32 [rows, nodes] (-1 behind them), the token after it int64
+    [rows]). ``tokens`` / ``choice`` int64 [rows, nodes]: the drafted tokens, and what the model writes after each; the path starts at node 0 and goes
+    on with the child whose token is the choice (the first of equal ones). Keys and values of its nodes go from ``drafts``
+    (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
+    itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out."""
+    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    L, B, Hkv, Smax, D = k_cache.shape
+    if tree.shape[0] != B or tuple(tokens.shape) != tuple(tree.shape) or tuple(choice.shape) != tuple(tree.shape):
+        raise ValueError(f"tree {tuple(tree.shape)}, tokens {tuple(tokens.shape)} and choice {tuple(choice.shape)} of {B} rows do not go together")
+    if tokens.dtype != torch.int64 or choice.dtype != torch.int64:
+        raise ValueError("tokens and choice: int64 expected")
+    if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or x.dtype != k_cache.dtype or x.shape[0] != B * tree.shape[1]
+                               or x.shape[1] % D or x.shape[1] <= 2 * Hkv * D for x in drafts):
+        raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")
+    kv_len = _ints(kv_len, "kv_len", (B,), k_cache)
+    if on_gpu(k_cache):
+        return tuple(native().tree_accept(tree.parent, tree.see, tokens.contiguous(), choice.contiguous(), drafts, k_cache, v_cache, kv_len))
+    return ref.tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len)

@@ -392,3 +392,96 @@ def moe_route(logits, correction, top, nshared, gate_col):
         idx = torch.cat([idx, torch.arange(E, E + nshared).expand(T, -1)], -1)
         w = torch.cat([w, gate.expand(T, nshared)], -1)
     return idx.int(), w.contiguous()
+
+
+# ------------------------------------------------------------------------------ drafted tokens
+def draft_tree(parent, nodes=None, pos0=None):
+    """-> (see int64 [B, N], pos int32 [B, N])"""
+    B, N = parent.shape
+    i = torch.arange(N, device=parent.device)
+    live = torch.ones(B, N, dtype=torch.bool, device=parent.device) if nodes is None else i[None] < nodes.long()[:, None]
+    p = torch.where(live & (parent >= 0) & (parent < i), parent.long(), i)
+    see = torch.ones((), dtype=torch.int64, device=parent.device) << i
+    see = see[None].repeat(B, 1)
+    depth = torch.zeros(B, N, dtype=torch.long, device=parent.device)
+    for k in range(1, N):  # parents come first
+        up = p[:, k:k + 1]
+        own = (up == k)[:, 0]
+        see[:, k] = torch.where(own, see[:, k], see[:, k] | see.gather(1, up)[:, 0])
+        depth[:, k] = torch.where(own, 0, depth.gather(1, up)[:, 0] + 1)
+    first = torch.zeros(B, dtype=torch.int32, device=parent.device) if pos0 is None else pos0
+    return torch.where(live, see, 0), (first[:, None] + torch.where(live, depth, 0)).int()
+
+
+def tree_attention(qkv, kc, vc, kv_len, see, Hq, kv_start=None, window=0, scale=None):
+    B, Hkv, Smax, D = kc.shape
+    N, G = see.shape[1], Hq // Hkv
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
+    x = qkv[:, :(Hq + 2 * Hkv) * D].to(wide).view(B, N, Hq + 2 * Hkv, D).transpose(1, 2)
+    out = torch.zeros(B, N, Hq, D, dtype=wide, device=qkv.device)
+    bits = [[[j for j in range(N) if s >> j & 1] for s in row] for row in see.tolist()]
+    for b in range(B):
+        n = min(max(int(kv_len[b]), 0), Smax)
+        lo = max(int(kv_start[b]), 0) if kv_start is not None else 0
+        for i in range(N):
+            mine = bits[b][i]
+            if not mine:
+                continue
+            first = max(lo, n + len(mine) - window) if window else lo
+            near = [j for j in mine if not window or len(mine) - len(bits[b][j]) < window]
+            k = torch.cat([kc[b, :, first:n].to(wide), x[b, Hq:Hq + Hkv, near]], 1)
+            v = torch.cat([vc[b, :, first:n].to(wide), x[b, Hq + Hkv:, near]], 1)
+            q = x[b, :Hq, i].view(Hkv, G, D)
+            p = torch.softmax(q @ k.transpose(1, 2) * scale, -1)
+            out[b, i] = (p @ v).reshape(Hq, D)
+    return out.view(B * N, Hq * D).to(qkv.dtype)
+
+
+def tree_accept(parent, see, tokens, choice, drafts, kc, vc, kv_len):
+    L, B, Hkv, Smax, D = kc.shape
+    N = see.shape[1]
+    count = torch.zeros(B, dtype=torch.int32, device=kc.device)
+    path = torch.full((B, N), -1, dtype=torch.int32, device=kc.device)
+    after = torch.full((B,), -1, dtype=torch.int64, device=kc.device)
+    up, tok, ch, live = parent.tolist(), tokens.tolist(), choice.tolist(), (see != 0).tolist()
+    for b in range(B):
+        nodes, cur = [], 0 if live[b][0] else -1
+        while cur >= 0:
+            nodes.append(cur)
+            cur = next((i for i in range(cur + 1, N) if live[b][i] and up[b][i] == cur and tok[b][i] == ch[b][cur]), -1)
+        if not nodes:
+            continue
+        count[b], after[b] = len(nodes), ch[b][nodes[-1]]
+        path[b, :len(nodes)] = torch.tensor(nodes, dtype=torch.int32)
+        at = max(int(kv_len[b]), 0)
+        nodes = nodes[:max(Smax - at, 0)]
+        for layer, x in enumerate(drafts):
+            rows = x.view(B, N, -1, D)[b, nodes].transpose(0, 1)
+            kc[layer, b, :, at:at + len(nodes)] = rows[-2 * Hkv:-Hkv]
+            vc[layer, b, :, at:at + len(nodes)] = rows[-Hkv:]
+    return count, path, after
+
+
+def alternatives(logits, targets, top, inv_temp=1.0):
+    """(log-probabilities of the targets, entropy, the best alternatives' log-probabilities, their ids); differentiable"""
+    T, V = logits.shape
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    raw = x.detach()
+    raw = torch.where(torch.isnan(raw), torch.full_like(raw, -math.inf), raw)
+    ids = torch.sort(raw, dim=1, descending=True, stable=True).indices[:, :top]
+    m = raw.amax(1, keepdim=True)
+    none = (x.detach() == -math.inf).all(1)  # no choice is left: no entropy and no gradient
+    z = torch.where(none[:, None], torch.zeros_like(x), (x - m) * inv_temp)
+    ls = torch.logsumexp(z, 1, keepdim=True)
+    logp = z - ls
+    p = torch.exp(logp)
+    ent = ls[:, 0] - torch.where(p == 0, torch.zeros_like(p), p * torch.where(p == 0, torch.zeros_like(z), z)).sum(1)
+    lost = torch.full_like(ent, -math.inf)
+    ent = torch.where(none, torch.zeros_like(ent), ent)
+    top_lp = torch.where(none[:, None], lost[:, None], logp.gather(1, ids))
+    if targets is None:
+        return torch.zeros_like(ent), ent, top_lp, ids
+    t = targets.long()
+    lp = torch.where(none, lost, logp.gather(1, t.clamp(min=0)[:, None])[:, 0])
+    return torch.where(t >= 0, lp, torch.zeros_like(lp)), ent, top_lp, ids
