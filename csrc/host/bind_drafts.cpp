@@ -9,8 +9,9 @@
 
 extern "C" {
 int rt_draft_tree(const int*, const int*, const int*, int, int, int64_t*, int*, hipStream_t);
-int rt_tree_attention(int, const void*, long, const void*, const void*, const int*, const int*, const int64_t*, void*, long, int, int, int, int,
-                      int, int, int, float, hipStream_t);
+int rt_tree_parts(int, int, int, int, int, int);
+int rt_tree_attention(int, const void*, long, const void*, const void*, const int*, const int*, const int64_t*, void*, long, float*, int, int,
+                      int, int, int, int, int, int, float, hipStream_t);
 int rt_tree_accept(const int*, const int64_t*, const int64_t*, const int64_t*, const int*, int*, int*, int64_t*, const void* const*, long, void*,
                    void*, long, int, int, int, int, int, int, int, int, hipStream_t);
 int rt_alternatives(int, const void*, long, const int64_t*, float, long, int, int, float*, float*, float*, int64_t*, float*, hipStream_t);
@@ -37,6 +38,7 @@ void act(const Tensor& t, const char* n) {
   TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat), n,
               ": GPU tensor of bf16 or fp32 expected");
 }
+bool al(const Tensor& t, uintptr_t n) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % n == 0; }
 void whole(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
   on(t, like, n);
   TORCH_CHECK(t.scalar_type() == type && t.sizes() == shape && t.is_contiguous(), n, ": contiguous ", type, " ", shape, " expected, got ",
@@ -70,11 +72,19 @@ void tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const
   TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && qkv.size(0) == B * N && qkv.size(1) >= (Hq + 2 * Hkv) * D, "tree_attention: qkv shape");
   on(out, qkv, "tree_attention out");
   TORCH_CHECK(out.scalar_type() == qkv.scalar_type() && out.size(0) == B * N && out.size(1) == Hq * D, "tree_attention: out shape");
-  TORCH_CHECK(Smax * D < (1L << 29) && window >= 0 && window < (1L << 30), "tree_attention: sizes");
+  TORCH_CHECK(Smax * D < (1L << 30) && window >= 0 && window < (1L << 30) && scale > 0, "tree_attention: sizes");
   const c10::DeviceGuard guard(qkv.device());
-  rc_ok(rt_tree_attention(qkv.scalar_type() == at::kFloat, qkv.data_ptr(), qkv.stride(0), kc.data_ptr(), vc.data_ptr(), kv_len.data_ptr<int>(),
-                          ptr<int>(kv_start), see.data_ptr<int64_t>(), out.data_ptr(), out.stride(0), (int)B, (int)N, (int)Hq, (int)Hkv, (int)D,
-                          (int)Smax, (int)window, (float)scale, stream()), "tree_attention");
+  const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
+                        ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax) : 0;
+  // matrix instructions want rows at 16 bytes (the output at 8): others are copied
+  Tensor x = qkv, o = out;
+  if (S && !(al(x, 16) && x.stride(0) % 8 == 0 && x.stride(0) < (1L << 24))) x = qkv.narrow(1, 0, (Hq + 2 * Hkv) * D).clone(at::MemoryFormat::Contiguous);
+  if (S && !(al(o, 8) && o.stride(0) % 4 == 0)) o = at::empty({B * N, Hq * D}, qkv.options());
+  Tensor part = S > 1 ? at::empty({S * B * Hq * N * (D + 2)}, qkv.options().dtype(at::kFloat)) : Tensor();
+  rc_ok(rt_tree_attention(x.scalar_type() == at::kFloat, x.data_ptr(), x.stride(0), kc.data_ptr(), vc.data_ptr(), kv_len.data_ptr<int>(),
+                          ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
+                          (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, stream()), "tree_attention");
+  if (!o.is_same(out)) out.copy_(o);
 }
 
 std::vector<Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens, const Tensor& choice,

@@ -4,6 +4,8 @@
 #include "rt_common.h"
 #include "rt_paged.h"
 
+#include <algorithm>
+
 namespace rt {
 namespace drafts {
 
@@ -50,6 +52,7 @@ struct TreeArgs {
   void* o; long ldo;
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
+  float* part; int S;                   // [S, B, Hkv, N Hq / Hkv, D + 2] partials (o | m | l) of at most S shares of a row's keys
 };
 
 template <typename T>
@@ -114,6 +117,334 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
     __syncthreads();
   }
   for (int c = tid; c < a.D; c += 256) st(o + c, acc[c] / l);  // a node sees itself
+}
+
+// ---------------------------------------------------------------------------------------------
+// attention in bf16 on matrix instructions
+// ---------------------------------------------------------------------------------------------
+// A workgroup takes one key head of a row: its queries (node r / G, head r % G of the group for row r of G N) against a share of the
+// keys, in stages of SK keys that go to LDS by DMA while the stage before is multiplied. The context comes from the cache; the nodes'
+// own keys are the last stage. S^T = K Q^T and O^T = V^T P^T: a query is a lane's column in both, so its maximum and sum lie in four
+// lanes, and p goes from the scores' registers to the product's as it is (rounded to the cache's type: half a step of bf16 for each term,
+// the sums in fp32). WR waves share the rows, RT tiles of 16 each, WK the keys of a stage.
+// Shares of a long row's keys (cut(): by the lengths, which only the device knows) leave fp32 partials that a second launch joins.
+struct Cut { int lo, len, tiles, parts, per; };  // tiles: stages of the context and the nodes' one
+__device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int SK) {
+  Cut c;
+  c.len = min(max(a.kv_len[b], 0), a.Smax);
+  c.lo = a.kv_start ? max(a.kv_start[b], 0) : 0;
+  if (a.window) c.lo = max(c.lo, c.len - a.window + 1);
+  c.lo = min(c.lo, c.len);
+  c.tiles = (c.len - c.lo + SK - 1) / SK + 1;
+  c.per = max((c.tiles + a.S - 1) / a.S, min(c.tiles, 2));
+  c.parts = (c.tiles + c.per - 1) / c.per;
+  return c;
+}
+
+// ancestors less than `window` positions before a node: the last ones
+__device__ __forceinline__ uint64_t near_nodes(uint64_t see, int window) {
+  if (window)
+    for (int far = __popcll(see) - window; far > 0; --far) see &= see - 1;
+  return see;
+}
+
+template <int D, int RT, int WR, int WK, int KT>
+__global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
+  constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
+  static_assert(KB / 1024 % NW == 0 && SK >= NODES);
+  __shared__ __attribute__((aligned(16))) char smem[4 * KB];
+  __shared__ unsigned bad[2];  // nodes whose values are not all numbers
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
+  const int s = blockIdx.x % a.S, pair = blockIdx.x / a.S % (a.B * a.Hkv), rb = blockIdx.x / a.S / (a.B * a.Hkv);
+  const int b = pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
+  const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
+  const uint64_t live = __ballot(see != 0);
+  const int n = live ? 64 - __builtin_clzll(live) : 0, M = n * G;
+  const Cut ct = cut(a, b, SK);
+  if (s >= ct.parts) return;
+  const int t0 = s * ct.per, t1 = min(t0 + ct.per, ct.tiles);
+  const int row0 = rb * ROWS + wr * 16 * RT;  // of this wave
+  const bf16_t* const x = (const bf16_t*)a.qkv + (long)b * a.N * a.ldq;
+
+  if (rb * ROWS < M) {
+    bf16x8 qf[RT][DS];
+    uint64_t sees[RT];
+    int from[RT];  // first key of the context that the row sees
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const int r = min(row0 + 16 * u + r16, M - 1), node = r / G;
+      const bf16_t* const q = x + (long)node * a.ldq + (long)(gh * G + r % G) * D + 8 * g;
+#pragma unroll
+      for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
+      const uint64_t w = lane64(see, node);
+      sees[u] = near_nodes(w, a.window);
+      from[u] = a.window ? ct.len + __popcll(w) - a.window : 0;
+    }
+    f32x4 o[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      m[u] = -INFINITY; l[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < DT; ++c) o[u][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const long head = ((long)b * a.Hkv + gh) * a.Smax * D;
+    auto stage = [&](int tile, int buf) {
+      const bool own = tile == ct.tiles - 1;
+      const bf16_t* const kb = own ? x + (long)(a.Hq + gh) * D : (const bf16_t*)a.kc + head;
+      const bf16_t* const vb = own ? x + (long)(a.Hq + a.Hkv + gh) * D : (const bf16_t*)a.vc + head;
+      const int first = own ? 0 : ct.lo + tile * SK, last = (own ? n : ct.len) - 1, pitch = own ? (int)a.ldq * 2 : D * 2;
+#pragma unroll
+      for (int j = 0; j < 2 * KB / 1024 / NW; ++j) {
+        const bool v = j >= KB / 1024 / NW;
+        const int at = (v ? j - KB / 1024 / NW : j) * NW + wid, e = at * 64 + lane, key = e / NC;
+        const int c = v ? paged::vv_chunk<D>(key, e % NC) : paged::kq_chunk<D>(key, e % NC);
+        // keys behind the last one repeat it: they are masked, and what lies there is nobody's
+        paged::lds_dma16(v ? vb : kb, (uint32_t)(min(first + key, last) * pitch + 16 * c), smem + (2 * buf + v) * KB + at * 1024);
+      }
+    };
+    if (tid < 2) bad[tid] = 0;
+    stage(t0, 0);
+    int cur = 0;
+    for (int t = t0; t < t1; ++t, cur ^= 1) {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
+      asm volatile("s_barrier" ::: "memory");           // ... by every wave; the other buffer is free
+      if (t + 1 < t1) stage(t + 1, cur ^ 1);
+      const bool own = t == ct.tiles - 1;
+      char* const Ks = smem + 2 * cur * KB + wk * KT * D * 2;
+      char* const Vs = smem + (2 * cur + 1) * KB + wk * KT * D * 2;
+      if (own) {
+        // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
+        // product and are added below for the rows that see them
+        char* const img = smem + (2 * cur + 1) * KB;
+        for (int e = tid; e < NODES * NC; e += 64 * NW) {
+          uint32_t* const w = (uint32_t*)(img + e * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+            if (lo || hi) {
+              w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+              atomicOr(&bad[e / NC / 32], 1u << (e / NC % 32));
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (row0 >= M) continue;
+      f32x4 st[KS][RT];
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int u = 0; u < RT; ++u) st[k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int d = 0; d < DS; ++d) {
+          // the swizzle goes by the row within the stage: KT rows are a multiple of its period
+          const bf16x8 kf = *(const bf16x8*)(Ks + paged::kq_off<D>(16 * k + r16, 4 * d + g));
+#pragma unroll
+          for (int u = 0; u < RT; ++u) st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][d], st[k][u], 0, 0, 0);
+        }
+      const int key0 = wk * KT + 4 * g;  // of the stage: this lane's keys are key0 + 16 k + e
+      if (own) {
+#pragma unroll
+        for (int u = 0; u < RT; ++u)
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            const unsigned bits = (unsigned)(sees[u] >> (key0 + 16 * k));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(bits >> e & 1)) st[k][u][e] = -INFINITY;
+          }
+      } else {
+        const int first = ct.lo + t * SK;
+        if (first + SK > ct.len || (a.window && first < ct.len + NODES - a.window)) {
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int key = first + key0 + 16 * k + e;
+                if (key >= ct.len || key < from[u]) st[k][u][e] = -INFINITY;
+              }
+        }
+      }
+      float alpha[RT];
+#pragma unroll
+      for (int u = 0; u < RT; ++u) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) mx = fmaxf(mx, fmaxf(fmaxf(st[k][u][0], st[k][u][1]), fmaxf(st[k][u][2], st[k][u][3])));
+        const float mn = fmaxf(m[u], over_groups(mx, [](float p, float q) { return fmaxf(p, q); }));
+        const float mz = (mn == -INFINITY ? 0.f : mn) * a.scale;  // a row may see nothing of its first stages
+        alpha[u] = paged::fexp2(m[u] * a.scale - mz);
+        m[u] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = paged::fexp2(fmaf(st[k][u][e], a.scale, -mz));
+            st[k][u][e] = p;
+            sum += p;
+          }
+        l[u] = l[u] * alpha[u] + sum;  // of this lane's keys; the four lanes are added at the end
+      }
+      bool grown = false;
+#pragma unroll
+      for (int u = 0; u < RT; ++u) grown = grown || alpha[u] != 1.f;
+      if (__any(grown)) {
+#pragma unroll
+        for (int u = 0; u < RT; ++u)
+#pragma unroll
+          for (int c = 0; c < DT; ++c) o[u][c] *= alpha[u];
+      }
+      bf16x8 pf[KT / 32][RT];
+#pragma unroll
+      for (int k = 0; k < KT / 32; ++k)
+#pragma unroll
+        for (int u = 0; u < RT; ++u) pf[k][u] = paged::pack_p(st[2 * k][u], st[2 * k + 1][u]);
+      const int key_a = 4 * g + (lane >> 2 & 3), pcol = lane & 3;  // transposed reads: rows 16 apart have the same swizzle
+#pragma unroll
+      for (int c = 0; c < DT; c += 4) {
+        uint32_t va[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) va[k] = lds_addr(Vs + paged::vv_off<D>(key_a, 2 * (c + k) + (pcol >> 1)) + ((pcol & 1) << 3));
+        if constexpr (KT == 64) {
+          rt_s16x4 v[16];
+          ds_tr16_frag4<16 * D * 2, 32 * D * 2, 48 * D * 2>(va[0], va[1], va[2], va[3], v);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bf16x8 vf = paged::cat4(v[4 * k + 2 * h], v[4 * k + 2 * h + 1]);
+#pragma unroll
+              for (int u = 0; u < RT; ++u) o[u][c + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[h][u], o[u][c + k], 0, 0, 0);
+            }
+        } else {
+          const uint32_t at[8] = {va[0], va[0] + 32 * D, va[1], va[1] + 32 * D, va[2], va[2] + 32 * D, va[3], va[3] + 32 * D};
+          rt_s16x4 v[8];
+          ds_tr16_at8(at, v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const bf16x8 vf = paged::cat4(v[2 * k], v[2 * k + 1]);
+#pragma unroll
+            for (int u = 0; u < RT; ++u) o[u][c + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[0][u], o[u][c + k], 0, 0, 0);
+          }
+        }
+      }
+      if (own) {
+        const uint64_t ill = ((uint64_t)bad[1] << 32 | bad[0]) & (KT == 64 ? ~0ull : 0xffffffffull << (wk * KT));
+        for (uint64_t w = ill; w; w &= w - 1) {
+          const int node = __builtin_ctzll(w);
+          const bf16_t* const v = x + (long)node * a.ldq + (long)(a.Hq + a.Hkv + gh) * D + 4 * g;
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+            if (sees[u] >> node & 1)
+#pragma unroll
+              for (int c = 0; c < DT; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float f = bf2f(v[16 * c + e]);
+                  if (!(fabsf(f) < INFINITY)) o[u][c][e] += f;
+                }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < RT; ++u) l[u] = over_groups(l[u], [](float p, float q) { return p + q; });
+    if constexpr (WK > 1) {  // the keys' shares, joined in order
+      float* const sh = (float*)smem;
+      for (int k = 1; k < WK; ++k) {
+        __syncthreads();
+        if (wk == k) {
+#pragma unroll
+          for (int u = 0; u < RT; ++u) {
+            float* const p = sh + ((wr * RT + u) * (DT * 4 + 2)) * 64 + lane;
+            p[0] = m[u];
+            p[64] = l[u];
+#pragma unroll
+            for (int c = 0; c < DT; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) p[(2 + 4 * c + e) * 64] = o[u][c][e];
+          }
+        }
+        __syncthreads();
+        if (wk == 0) {
+#pragma unroll
+          for (int u = 0; u < RT; ++u) {
+            const float* const p = sh + ((wr * RT + u) * (DT * 4 + 2)) * 64 + lane;
+            const float mn = fmaxf(m[u], p[0]), mz = (mn == -INFINITY ? 0.f : mn) * a.scale;
+            const float x0 = paged::fexp2(m[u] * a.scale - mz), x1 = paged::fexp2(p[0] * a.scale - mz);
+            m[u] = mn;
+            l[u] = l[u] * x0 + p[64] * x1;
+#pragma unroll
+            for (int c = 0; c < DT; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[u][c][e] = o[u][c][e] * x0 + p[(2 + 4 * c + e) * 64] * x1;
+          }
+        }
+      }
+      if (wk) return;
+    }
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const int r = row0 + 16 * u + r16;
+      if (r >= M) continue;
+      if (ct.parts > 1) {
+        float* const p = a.part + (((long)s * a.B + b) * a.Hkv + gh) * ((long)a.N * G * (D + 2)) + (long)r * (D + 2);
+        if (g == 0) { p[D] = m[u] * a.scale; p[D + 1] = l[u]; }
+#pragma unroll
+        for (int c = 0; c < DT; ++c) {
+          *(float2*)(p + 16 * c + 4 * g) = make_float2(o[u][c][0], o[u][c][1]);
+          *(float2*)(p + 16 * c + 4 * g + 2) = make_float2(o[u][c][2], o[u][c][3]);
+        }
+      } else {
+        const float inv = 1.f / l[u];  // a node sees itself
+        bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 4 * g;
+#pragma unroll
+        for (int c = 0; c < DT; ++c)
+          *(uint2*)(p + 16 * c) = make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv));
+      }
+    }
+  }
+  if (s == 0) {  // rows that are no nodes
+    for (int r = max(M, rb * ROWS) + wid; r < min(a.N * G, (rb + 1) * ROWS); r += NW) {
+      bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D;
+      if (lane < D / 4) *(uint2*)(p + 4 * lane) = make_uint2(0, 0);
+    }
+  }
+}
+
+// the parts of rows that were cut, one wave a (node, head)
+template <int D>
+__global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
+  const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv, per = a.N * G;
+  const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6), pair = w / per;
+  const int r = (int)(w % per);
+  if (pair >= (long)a.B * a.Hkv) return;
+  const int b = (int)(pair / a.Hkv), gh = (int)(pair % a.Hkv);
+  if (!a.see[(long)b * a.N + r / G]) return;
+  const Cut ct = cut(a, b, SK);
+  if (ct.parts == 1) return;
+  const long step = (long)a.B * a.Hkv * per * (D + 2);
+  const float* const p = a.part + (pair * per + r) * (D + 2);
+  float m = -INFINITY, l = 0.f, o[D / 64];
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
+  for (int s = 0; s < ct.parts; ++s) {
+    const float* const q = p + s * step;
+    const float ms = q[D], mn = fmaxf(m, ms), mz = mn == -INFINITY ? 0.f : mn;
+    const float x0 = paged::fexp2(m - mz), x1 = paged::fexp2(ms - mz);
+    m = mn;
+    l = l * x0 + q[D + 1] * x1;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) o[i] = o[i] * x0 + q[D / 64 * lane + i] * x1;
+  }
+  bf16_t* const out = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + D / 64 * lane;
+  if constexpr (D == 128) *(uint32_t*)out = pack2bf(o[0] / l, o[1] / l);
+  else out[0] = f2bf(o[0] / l);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -189,16 +520,53 @@ extern "C" int rt_draft_tree(const int* parent, const int* nodes, const int* pos
   return 0;
 }
 
+template <int D, int RT, int WR, int WK, int KT>
+static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
+  const int blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
+  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), dim3((unsigned)(a.S * a.B * a.Hkv * blocks)), dim3(64 * WR * WK), 0, stream, a);
+}
+template <int D>
+static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
+  if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32>(a, rows, stream);
+  else if (rows <= 32) launch_tree_form<D, 1, 2, 1, 64>(a, rows, stream);
+  else if (rows <= 64) launch_tree_form<D, 1, 4, 1, 64>(a, rows, stream);
+  else if (rows <= 128) launch_tree_form<D, 2, 4, 1, 64>(a, rows, stream);
+  else launch_tree_form<D, 2, 8, 1, 64>(a, rows, stream);
+  RT_LAUNCH_CHECK();
+  return 0;
+}
+
+// parts that a row's keys may be cut in: the partials that rt_tree_attention wants. 0: sizes without matrix instructions
+extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax) {
+  if ((D != 64 && D != 128) || B == 0) return 0;
+  const int stages = (Smax + 63) / 64 + 1, blocks = B * Hkv * ((N * (Hq / Hkv) + 255) / 256);
+  return std::max(1, std::min((2 * num_cus() + blocks - 1) / blocks, (stages + 1) / 2));
+}
+
 extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const int* kv_len, const int* kv_start,
-                                 const int64_t* see, void* o, long ldo, int B, int N, int Hq, int Hkv, int D, int Smax, int window,
-                                 float scale, hipStream_t stream) {
+                                 const int64_t* see, void* o, long ldo, float* part, int S, int B, int N, int Hq, int Hkv, int D, int Smax,
+                                 int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  const TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale};
-  const size_t shm = (2 * D + 256 + 4) * sizeof(float);
-  if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
-  else hipLaunchKernelGGL(tree_any_kernel<bf16_t>, dim3(N, Hq, B), dim3(256), shm, stream, a);
-  RT_LAUNCH_CHECK();
+  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, part, S};
+  if (S < 1) {
+    const size_t shm = (2 * D + 256 + 4) * sizeof(float);
+    if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
+    else hipLaunchKernelGGL(tree_any_kernel<bf16_t>, dim3(N, Hq, B), dim3(256), shm, stream, a);
+    RT_LAUNCH_CHECK();
+    return 0;
+  }
+  if (f32 || (D != 64 && D != 128) || (S > 1 && !part)) return -1;
+  a.scale = scale * 1.4426950408889634f;
+  const int rows = N * (Hq / Hkv);
+  const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
+  if (rc) return rc;
+  if (S > 1) {
+    const dim3 grid((unsigned)(((long)B * Hkv * rows + 3) / 4));
+    if (D == 128) hipLaunchKernelGGL(tree_join_kernel<128>, grid, dim3(256), 0, stream, a, 64);
+    else hipLaunchKernelGGL(tree_join_kernel<64>, grid, dim3(256), 0, stream, a, 64);
+    RT_LAUNCH_CHECK();
+  }
   return 0;
 }
 

@@ -69,11 +69,11 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"{Hq} heads over {Hkv} of {D} do not fit {qkv.shape[1]} columns")
     if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
         raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}: an fp8 cache is read by decode_step_attention only")
-    if window < 0:
-        raise ValueError(f"window {window}")
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if window < 0 or not scale > 0:
+        raise ValueError(f"window {window}, scale {scale}")
     kv_len = _ints(kv_len, "kv_len", (B,), qkv)
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
-    scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if out is None:
         out = torch.empty(B * N, Hq * D, dtype=qkv.dtype, device=qkv.device)
     if on_gpu(qkv):
