@@ -24,106 +24,275 @@ __device__ __forceinline__ uint64_t order(float v, int i) {
   return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (uint32_t)~i;
 }
 
-// of a part of the row: largest l, sum exp z, sum exp(z) z (m = -inf: nothing but -inf and NaN, which make the sums NaN)
-struct Sums { float m, s, t; };
-__device__ __forceinline__ Sums merge(Sums a, Sums b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  auto part = [&](Sums& p) {
-    if (p.m == m || p.m == -INFINITY) return;
-    const float d = c * (p.m - m), e = __expf(d);
-    p.t = e > 0.f ? e * (p.t + d * p.s) : 0.f * p.s;  // d may be -inf
-    p.s *= e;
-  };
-  part(a); part(b);
-  return Sums{m, a.s + b.s, a.t + b.t};
+// 16 bytes of a row, wherever they start: rows of an odd pitch need no copy (loads take any address)
+template <typename T> struct Chunk;
+template <> struct Chunk<bf16_t> {
+  static constexpr int E = 8;
+  static __device__ __forceinline__ void open(const u32x4& w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint32_t word(const bf16_t* p, int n, int i) {  // word i of a chunk with n elements left
+    const uint32_t none = 0xff80u;  // -inf
+    return (2 * i < n ? (uint32_t)p[2 * i] : none) | (2 * i + 1 < n ? (uint32_t)p[2 * i + 1] : none) << 16;
+  }
+};
+template <> struct Chunk<float> {
+  static constexpr int E = 4;
+  static __device__ __forceinline__ void open(const u32x4& w, float* f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+  }
+  static __device__ __forceinline__ uint32_t word(const float* p, int n, int i) { return i < n ? __float_as_uint(p[i]) : 0xff800000u; }
+};
+// the chunk behind the last whole one: -inf past the row
+template <typename T>
+__device__ __forceinline__ u32x4 load_tail(const T* x, int c, int V) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = Chunk<T>::word(x + (long)c * Chunk<T>::E, V - c * Chunk<T>::E, i);
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 load_chunk(const T* x, int c, int V) {
+  u32x4 w;
+  if ((c + 1) * Chunk<T>::E <= V) __builtin_memcpy(&w, x + (long)c * Chunk<T>::E, 16);
+  else w = load_tail(x, c, V);
+  return w;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void alternatives_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
-                                                           int V, int top, float* __restrict__ logp, float* __restrict__ ent,
-                                                           float* __restrict__ top_lp, int64_t* __restrict__ ids, float* __restrict__ stats) {
-  __shared__ float sm[4][3];
-  __shared__ uint64_t best[4];
+constexpr int CAP = 512;       // candidates that are ranked at once
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// One workgroup a row, which stays in registers: NC chunks a thread (0: it does not fit, and is read again from the caches).
+// The alternatives without sorting: the best of each lane's elements over the waves makes 64 numbers of which no two are equal (value,
+// then place), and the top-th of them is one that at least `top` elements reach. What reaches it is a little more than `top` elements (24 of 32000
+// where 20 are wanted); each counts how many of the others are before it. Where they are more than CAP (rows made for it) the
+// best are taken one by one.
+template <typename T, int THREADS, int NC>
+__global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
+                                                               int V, int top, float* __restrict__ logp, float* __restrict__ ent,
+                                                               float* __restrict__ top_lp, int64_t* __restrict__ ids,
+                                                               float* __restrict__ stats) {
+  constexpr int E = Chunk<T>::E, NW = THREADS / 64, KEEP = NC ? NC : 1;
+  __shared__ float sm[3][NW];
+  __shared__ uint64_t best[THREADS], cand[CAP], tau_s;
+  __shared__ int count;
   const long row = blockIdx.x;
   const T* const x = logits + row * ld;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  Sums a{-INFINITY, 0.f, 0.f};
-  for (int i = tid; i < V; i += 256) {
-    const float f = get(x + i);
-    if (f != f) a.s += f;
-    else if (f > -INFINITY) a = merge(a, Sums{f, f == INFINITY ? NAN : 1.f, 0.f}, c);
-  }
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, chunks = (V + E - 1) / E;
+  u32x4 data[KEEP];
+  float top_of[KEEP];
+  if constexpr (NC > 0) {
+    const uint32_t none = E == 8 ? 0xff80ff80u : 0xff800000u;  // -inf: counts for nothing
+    const int full = V / E;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    a = merge(a, Sums{__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.t, off, 64)}, c);
-  if (lane == 0) { sm[wid][0] = a.m; sm[wid][1] = a.s; sm[wid][2] = a.t; }
+    for (int k = 0; k < NC; ++k) {
+      const int ch = k * THREADS + tid;
+      data[k] = u32x4{none, none, none, none};
+      if (ch < full) __builtin_memcpy(&data[k], x + (long)ch * E, 16);
+    }
+    if (full < chunks && tid == full % THREADS) {
+      const u32x4 w = load_tail(x, full, V);
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+        if (k == full / THREADS) data[k] = w;
+    }
+  }
+  // f(turn, chunk, its elements) for the thread's chunks in order
+  auto each = [&](auto f) {
+    if constexpr (NC > 0) {
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        asm volatile("" : "+v"(data[k]));  // opened anew in each pass: kept open it takes twice the registers
+        f(k, k * THREADS + tid, data[k]);
+      }
+    } else {
+      for (int ch = tid; ch < chunks; ch += THREADS) f(0, ch, load_chunk(x, ch, V));
+    }
+  };
+  // the row's largest, and each thread's with the chunk where it lies
+  float mine = -INFINITY;
+  int where = tid;
+  each([&](int k, int ch, const u32x4& w) {
+    float f[E];
+    Chunk<T>::open(w, f);
+    float mx = -INFINITY;  // a NaN counts as this
+#pragma unroll
+    for (int i = 0; i < E; ++i) mx = fmaxf(mx, f[i]);
+    top_of[k] = mx;
+    if (mx > mine) { mine = mx; where = ch; }
+  });
+  best[tid] = tid < chunks ? order(mine, where) : 0;
+  const float wm = wave_max(mine);
+  if (lane == 0) sm[0][wid] = wm;
+  if (tid == 0) count = 0;
   __syncthreads();
-  a = Sums{sm[0][0], sm[0][1], sm[0][2]};
-  for (int w = 1; w < 4; ++w) a = merge(a, Sums{sm[w][0], sm[w][1], sm[w][2]}, c);
-  const bool none = a.m == -INFINITY && a.s == 0.f;
-  const float ls = none ? 0.f : __logf(a.s), mean = none ? 0.f : a.t / a.s;
-  auto log_prob = [&](float l) { return none ? -INFINITY : (l - a.m) * c - ls; };
+  float m = sm[0][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, sm[0][w]);
+  // the sums, in steps of log 2
+  const float c2 = c * LOG2E, ref = m == -INFINITY ? 0.f : m;
+  float s = 0.f, t = 0.f;
+  each([&](int, int, const u32x4& w) {
+    float f[E];
+    Chunk<T>::open(w, f);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = (f[i] - ref) * c2, e = __builtin_amdgcn_exp2f(z);
+      s += e;
+      t = fmaf(e, fmaxf(z, -1e30f), t);  // 0 for an element of -inf
+    }
+  });
+  s = wave_sum(s);
+  t = wave_sum(t);
+  if (lane == 0) { sm[1][wid] = s; sm[2][wid] = t; }
+  // the bound for the alternatives: wave 0, while the others go to the barrier
+  if (wid == 0) {
+    uint64_t b = best[lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) b = max(b, best[w * 64 + lane]);
+    const uint32_t lo = (uint32_t)b, hi = (uint32_t)(b >> 32);
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, j) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, j);
+      before += o > b;
+    }
+    if (b && before == top - 1) tau_s = b;
+    // fewer lanes with elements than alternatives: everything is ranked
+    if (__popcll(__ballot(b != 0)) < top && lane == 0) tau_s = 0;
+  }
+  __syncthreads();
+  s = sm[1][0];
+  t = sm[2][0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) { s += sm[1][w]; t += sm[2][w]; }
+  const bool none = m == -INFINITY && s == 0.f;
+  const float ls = none ? 0.f : __logf(s), mean = none ? 0.f : t / s * LN2;
+  auto log_prob = [&](float l) { return none ? -INFINITY : (l - ref) * c2 * LN2 - ls; };
   if (tid == 0) {
-    const int64_t t = tgt ? tgt[row] : -1;
-    logp[row] = t < 0 ? 0.f : t >= V ? NAN : log_prob(get(x + t));
+    const int64_t g = tgt ? tgt[row] : -1;
+    logp[row] = g < 0 ? 0.f : g >= V ? NAN : log_prob(get(x + g));
     ent[row] = ls - mean;
-    if (stats) { stats[row * 3] = none ? INFINITY : a.m; stats[row * 3 + 1] = ls; stats[row * 3 + 2] = mean; }
+    if (stats) { stats[row * 3] = none ? INFINITY : ref; stats[row * 3 + 1] = ls; stats[row * 3 + 2] = mean; }
+  }
+  const uint64_t tau = tau_s;
+  const uint32_t tu = (uint32_t)(tau >> 32);
+  const float tv = tau ? __uint_as_float(tu & 0x80000000u ? tu ^ 0x80000000u : ~tu) : -INFINITY;
+  each([&](int k, int ch, const u32x4& w) {
+    if (NC > 0 && !(top_of[k] >= tv)) return;
+    float f[E];
+    Chunk<T>::open(w, f);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (ch * E + i < V && order(f[i], ch) >= tau) {
+        const int at = atomicAdd(&count, 1);
+        if (at < CAP) cand[at] = order(f[i], ch * E + i);
+      }
+  });
+  __syncthreads();
+  const int n = count;
+  if (n <= CAP) {
+    for (int i = tid; i < n; i += THREADS) {
+      const uint64_t o = cand[i];
+      int before = 0;
+      for (int j = 0; j < n; ++j) before += cand[j] > o;
+      if (before < top) {
+        const int id = (int)~(uint32_t)o;
+        ids[row * top + before] = id;
+        top_lp[row * top + before] = log_prob(get(x + id));
+      }
+    }
+    return;
   }
   uint64_t last = ~0ull;
-  for (int k = 0; k < top; ++k) {  // the largest below the last one
+  for (int q = 0; q < top; ++q) {  // the largest behind the last one
     uint64_t b = 0;
-    for (int i = tid; i < V; i += 256) {
+    for (int i = tid; i < V; i += THREADS) {
       const uint64_t o = order(get(x + i), i);
       if (o < last && o > b) b = o;
     }
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const uint64_t o = __shfl_xor((unsigned long long)b, off, 64);
-      b = o > b ? o : b;
-    }
+    for (int off = 32; off > 0; off >>= 1) b = max(b, (uint64_t)__shfl_xor((unsigned long long)b, off, 64));
     __syncthreads();
     if (lane == 0) best[wid] = b;
     __syncthreads();
-    last = max(max(best[0], best[1]), max(best[2], best[3]));
+    last = best[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) last = max(last, best[w]);
     if (tid == 0) {
       const int id = (int)~(uint32_t)last;
-      ids[row * top + k] = id;
-      top_lp[row * top + k] = log_prob(get(x + id));
+      ids[row * top + q] = id;
+      top_lp[row * top + q] = log_prob(get(x + id));
     }
   }
 }
 
-// dl = c (up - p (sum up) - g_H p (z - mean)), up: the given token's and the alternatives' gradients at their places
+// dl = c (up - p (sum up) - g_H p (z - mean)), up: the given token's and the alternatives' gradients at their places. A row is read and
+// written once; the few chunks with such places are known by a bit of their index (others may share it: they look and find nothing).
 template <typename T>
 __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
                                                                int V, int top, const int64_t* __restrict__ ids,
                                                                const float* __restrict__ stats, const float* __restrict__ g_lp,
                                                                const float* __restrict__ g_ent, const float* __restrict__ g_top,
                                                                T* __restrict__ d, long ldd) {
+  constexpr int E = Chunk<T>::E, MARKS = 4096;
   __shared__ int at[MAX_TOP + 1];
   __shared__ float up[MAX_TOP + 1];
+  __shared__ unsigned marks[MARKS / 32];
   const long row = blockIdx.x;
   const T* const x = logits + row * ld;
   T* const dx = d + row * ldd;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, chunks = (V + E - 1) / E;
   const float m = stats[row * 3], ls = stats[row * 3 + 1], mean = stats[row * 3 + 2];
+  if (tid < MARKS / 32) marks[tid] = 0;
+  __syncthreads();
   if (tid <= top) {
-    const int64_t t = tgt ? tgt[row] : -1;
-    const bool given = tid < top || (t >= 0 && t < V);
-    at[tid] = !given ? -1 : tid < top ? (int)ids[row * top + tid] : (int)t;
+    const int64_t t = tid < top ? ids[row * top + tid] : tgt ? tgt[row] : -1;
+    const bool given = t >= 0 && t < V;
+    at[tid] = given ? (int)t : -1;
     up[tid] = !given ? 0.f : tid < top ? (g_top ? g_top[row * top + tid] : 0.f) : (g_lp ? g_lp[row] : 0.f);
+    if (given) atomicOr(&marks[(int)t / E % MARKS / 32], 1u << (t / E % 32));
   }
   __syncthreads();
   float total = 0.f;
   for (int k = 0; k <= top; ++k) total += up[k];
-  const float ge = g_ent ? g_ent[row] : 0.f;
+  const float ge = g_ent ? g_ent[row] : 0.f, c2 = c * LOG2E, ls2 = ls * LOG2E;
   const bool none = m == INFINITY && ls == 0.f;
-  for (int i = tid; i < V; i += 256) {
-    const float z = (get(x + i) - m) * c, p = __expf(z - ls);
-    float o = z == -INFINITY ? 0.f : -p * (total + ge * (z - mean));
-    for (int k = 0; k <= top; ++k)
-      if (at[k] == i) o += up[k];
-    put(dx + i, none ? 0.f : o * c);
+  // -c p (total + g_H (z - mean)) with z in steps of log 2
+  const float k1 = none ? 0.f : -c * (total - ge * mean), k2 = none ? 0.f : -c * ge * LN2;
+  for (int ch = tid; ch < chunks; ch += 256) {
+    float f[E];
+    Chunk<T>::open(load_chunk(x, ch, V), f);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float z = (f[i] - m) * c2, p = __builtin_amdgcn_exp2f(z - ls2);
+      f[i] = p * fmaf(k2, fmaxf(z, -1e30f), k1);
+    }
+    if (marks[ch % MARKS / 32] >> (ch % 32) & 1) {
+      for (int k = 0; k <= top; ++k) {
+        const int i0 = at[k] - ch * E;
+        if (at[k] >= 0 && i0 >= 0 && i0 < E)
+#pragma unroll
+          for (int i = 0; i < E; ++i) f[i] += i == i0 && !none ? c * up[k] : 0.f;
+      }
+    }
+    if ((ch + 1) * E <= V) {
+      if constexpr (E == 8) {
+        const uint4 w = pack8(f);
+        __builtin_memcpy(dx + (long)ch * E, &w, 16);
+      } else {
+        __builtin_memcpy(dx + (long)ch * E, f, 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (ch * E + i < V) put(dx + (long)ch * E + i, f[i]);
+    }
   }
 }
 
@@ -133,18 +302,32 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
 using namespace rt;
 using namespace rt::alt;
 
+template <typename T>
+static int launch_alternatives(const T* x, long ld, const int64_t* tgt, float c, long rows, int V, int top, float* logp, float* ent, float* top_lp,
+                               int64_t* ids, float* stats, hipStream_t stream) {
+  const int chunks = (V + Chunk<T>::E - 1) / Chunk<T>::E;
+#define ALT(THREADS, NC)                                                                                                                 \
+  hipLaunchKernelGGL((alternatives_kernel<T, THREADS, NC>), dim3((unsigned)rows), dim3(THREADS), 0, stream, x, ld, tgt, c, V, top, logp, ent, \
+                     top_lp, ids, stats)
+  const bool few = rows <= num_cus();  // a row a CU: as many threads as the row feeds
+  if (chunks <= 256 * 4) ALT(256, 4);
+  else if (few && chunks <= 1024 * 4) ALT(1024, 4);
+  else if (!few && chunks <= 256 * 16) ALT(256, 16);
+  else if (!few && chunks <= 512 * 16) ALT(512, 16);
+  else if (chunks <= 1024 * 8) ALT(1024, 8);
+  else if (chunks <= 1024 * 16) ALT(1024, 16);
+  else ALT(1024, 0);
+#undef ALT
+  RT_LAUNCH_CHECK();
+  return 0;
+}
+
 extern "C" int rt_alternatives(int f32, const void* logits, long ld, const int64_t* tgt, float c, long T, int V, int top, float* logp, float* ent,
                                float* top_lp, int64_t* ids, float* stats, hipStream_t stream) {
   if (T == 0) return 0;
   if (top < 1 || top > MAX_TOP || top > V) return -1;
-  if (f32)
-    hipLaunchKernelGGL(alternatives_kernel<float>, dim3(T), dim3(256), 0, stream, (const float*)logits, ld, tgt, c, V, top, logp, ent, top_lp,
-                       ids, stats);
-  else
-    hipLaunchKernelGGL(alternatives_kernel<bf16_t>, dim3(T), dim3(256), 0, stream, (const bf16_t*)logits, ld, tgt, c, V, top, logp, ent, top_lp,
-                       ids, stats);
-  RT_LAUNCH_CHECK();
-  return 0;
+  return f32 ? launch_alternatives((const float*)logits, ld, tgt, c, T, V, top, logp, ent, top_lp, ids, stats, stream)
+             : launch_alternatives((const bf16_t*)logits, ld, tgt, c, T, V, top, logp, ent, top_lp, ids, stats, stream);
 }
 
 extern "C" int rt_alternatives_bwd(int f32, const void* logits, long ld, const int64_t* tgt, float c, long T, int V, int top, const int64_t* ids,

@@ -257,6 +257,22 @@ def test_alternatives_of_rows_with_a_pattern(V, dtype):
         _check_alternatives(x, t, top, 1 / 0.7, grad=top == 8)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [9000, 32002, 50272, 70001, 140001])
+def test_alternatives_of_many_rows_are_those_of_few(V, dtype):
+    """more rows than CUs take other forms than a few do; random rows, and rows whose best lie in one thread's or one wave's share"""
+    i = torch.arange(V, device=DEV).float()
+    x = torch.cat([_rand(20, V, dtype=F32, seed=V) * 3, torch.stack([0 * i, i / V, (i // 8 % 256 == 7) * 9.0 - i / V, (i // 4 % 512 == 9) * 9.0 + i / V,
+                                                                     (i // 8 % 1024 == 2) * 9.0, torch.where(i == V - 2, 1.0, -math.inf)])]).to(dtype)
+    t = torch.arange(len(x), device=DEV)
+    few = ops.token_alternatives(x, t, 20, 1 / 0.7)
+    many = ops.token_alternatives(x.repeat(14, 1), t.repeat(14), 20, 1 / 0.7)
+    assert torch.equal(many[3], few[3].repeat(14, 1))
+    for a, b in zip(many[:3], few):  # other orders of the sums: 2^-23 (V / 256 + 16) each, of values below 16, and twice that of E|z|
+        b = b.repeat(14, *[1] * (b.dim() - 1))
+        assert ((a == b) | ((a - b).abs() <= 16 * 2 ** -23 * (V / 256 + 16))).all()
+
+
 def test_alternatives_of_rows_that_are_no_numbers():
     x = _rand(4, 600, seed=1)
     x[0, 300], x[1, :], x[2, 17], x[3, 599] = math.nan, math.nan, math.inf, math.nan
