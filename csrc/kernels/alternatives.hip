@@ -7,6 +7,8 @@
 // their order. A row of -inf alone has log-probabilities of -inf, no entropy and no gradient.
 #include "rt_common.h"
 
+#include <algorithm>
+
 namespace rt {
 namespace alt {
 
@@ -239,7 +241,7 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
                                                                int V, int top, const int64_t* __restrict__ ids,
                                                                const float* __restrict__ stats, const float* __restrict__ g_lp,
                                                                const float* __restrict__ g_ent, const float* __restrict__ g_top,
-                                                               T* __restrict__ d, long ldd) {
+                                                               T* __restrict__ d, long ldd, int span) {
   constexpr int E = Chunk<T>::E, MARKS = 4096;
   __shared__ int at[MAX_TOP + 1];
   __shared__ float up[MAX_TOP + 1];
@@ -265,9 +267,9 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
   const bool none = m == INFINITY && ls == 0.f;
   // -c p (total + g_H (z - mean)) with z in steps of log 2
   const float k1 = none ? 0.f : -c * (total - ge * mean), k2 = none ? 0.f : -c * ge * LN2;
-  for (int ch = tid; ch < chunks; ch += 256) {
+  auto one = [&](int ch, const u32x4& w) {
     float f[E];
-    Chunk<T>::open(load_chunk(x, ch, V), f);
+    Chunk<T>::open(w, f);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const float z = (f[i] - m) * c2, p = __builtin_amdgcn_exp2f(z - ls2);
@@ -293,7 +295,17 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
       for (int i = 0; i < E; ++i)
         if (ch * E + i < V) put(dx + (long)ch * E + i, f[i]);
     }
+  };
+  const int first = blockIdx.y * span, last = min(first + span, chunks);
+  int ch = first + tid;
+  for (; ch + 3 * 256 < min(last, V / E); ch += 4 * 256) {
+    u32x4 w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) __builtin_memcpy(&w[k], x + (long)(ch + k * 256) * E, 16);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) one(ch + k * 256, w[k]);
   }
+  for (; ch < last; ch += 256) one(ch, load_chunk(x, ch, V));
 }
 
 }  // namespace alt
@@ -330,17 +342,25 @@ extern "C" int rt_alternatives(int f32, const void* logits, long ld, const int64
              : launch_alternatives((const bf16_t*)logits, ld, tgt, c, T, V, top, logp, ent, top_lp, ids, stats, stream);
 }
 
+template <typename T>
+static int launch_alternatives_bwd(const T* x, long ld, const int64_t* tgt, float c, long rows, int V, int top, const int64_t* ids,
+                                   const float* stats, const float* g_lp, const float* g_ent, const float* g_top, T* d, long ldd,
+                                   hipStream_t stream) {
+  // a row goes to several workgroups where rows are few: eight of them a CU, with four chunks a thread at least
+  const int chunks = (V + Chunk<T>::E - 1) / Chunk<T>::E;
+  const int parts = (int)std::max(1L, std::min((8L * num_cus() + rows - 1) / rows, (long)(chunks + 1023) / 1024));
+  const int span = ((chunks + parts - 1) / parts + 255) / 256 * 256;
+  hipLaunchKernelGGL(alternatives_bwd_kernel<T>, dim3((unsigned)rows, (unsigned)((chunks + span - 1) / span)), dim3(256), 0, stream, x, ld, tgt, c,
+                     V, top, ids, stats, g_lp, g_ent, g_top, d, ldd, span);
+  RT_LAUNCH_CHECK();
+  return 0;
+}
+
 extern "C" int rt_alternatives_bwd(int f32, const void* logits, long ld, const int64_t* tgt, float c, long T, int V, int top, const int64_t* ids,
                                    const float* stats, const float* g_lp, const float* g_ent, const float* g_top, void* d, long ldd,
                                    hipStream_t stream) {
   if (T == 0) return 0;
   if (top < 1 || top > MAX_TOP || top > V) return -1;
-  if (f32)
-    hipLaunchKernelGGL(alternatives_bwd_kernel<float>, dim3(T), dim3(256), 0, stream, (const float*)logits, ld, tgt, c, V, top, ids, stats, g_lp,
-                       g_ent, g_top, (float*)d, ldd);
-  else
-    hipLaunchKernelGGL(alternatives_bwd_kernel<bf16_t>, dim3(T), dim3(256), 0, stream, (const bf16_t*)logits, ld, tgt, c, V, top, ids, stats,
-                       g_lp, g_ent, g_top, (bf16_t*)d, ldd);
-  RT_LAUNCH_CHECK();
-  return 0;
+  return f32 ? launch_alternatives_bwd((const float*)logits, ld, tgt, c, T, V, top, ids, stats, g_lp, g_ent, g_top, (float*)d, ldd, stream)
+             : launch_alternatives_bwd((const bf16_t*)logits, ld, tgt, c, T, V, top, ids, stats, g_lp, g_ent, g_top, (bf16_t*)d, ldd, stream);
 }
