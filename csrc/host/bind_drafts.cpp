@@ -5,6 +5,8 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <cmath>
+#include <tuple>
 #include <vector>
 
 extern "C" {
@@ -32,48 +34,66 @@ bool has(const optional<Tensor>& t) { return t.has_value() && t->defined(); }
 template <typename T> T* ptr(const optional<Tensor>& t) { return has(t) ? t->data_ptr<T>() : nullptr; }
 
 void on(const Tensor& t, const Tensor& like, const char* n) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), n, ": expected on ", like.device());
+  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device(), n, ": expected on ", like.device());
 }
 void act(const Tensor& t, const char* n) {
-  TORCH_CHECK(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat), n,
+  TORCH_CHECK_VALUE(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat), n,
               ": GPU tensor of bf16 or fp32 expected");
 }
 bool al(const Tensor& t, uintptr_t n) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % n == 0; }
 void whole(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
   on(t, like, n);
-  TORCH_CHECK(t.scalar_type() == type && t.sizes() == shape && t.is_contiguous(), n, ": contiguous ", type, " ", shape, " expected, got ",
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.sizes() == shape && t.is_contiguous(), n, ": contiguous ", type, " ", shape, " expected, got ",
               t.scalar_type(), " ", t.sizes());
 }
 
-std::vector<Tensor> draft_tree(const Tensor& parent, const optional<Tensor>& nodes, const optional<Tensor>& pos0) {
-  TORCH_CHECK(parent.is_cuda() && parent.dim() == 2, "draft_tree: parent [rows, nodes]");
-  const int64_t B = parent.size(0), N = parent.size(1);
-  whole(parent, at::kInt, {B, N}, parent, "draft_tree parent");
-  for (const auto* t : {&nodes, &pos0})
-    if (has(*t)) whole(**t, at::kInt, {B}, parent, "draft_tree nodes / pos0");
+// whole numbers of a row each, contiguous
+Tensor ints(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
+  on(t, like, n);
+  TORCH_CHECK_VALUE(t.scalar_type() == type && t.sizes() == shape, n, ": ", type, " ", shape, " expected, got ", t.scalar_type(), " ", t.sizes());
+  return t.contiguous();
+}
+optional<Tensor> ints(const optional<Tensor>& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
+  if (!has(t)) return c10::nullopt;
+  return ints(*t, type, shape, like, n);
+}
+
+std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parent_, const optional<Tensor>& nodes_, const optional<Tensor>& pos0_) {
+  TORCH_CHECK_VALUE(parent_.is_cuda() && parent_.dim() == 2 && parent_.size(1) >= 1 && parent_.size(1) <= 64,
+                    "parent: [rows, 1 .. 64 nodes] expected, got ", parent_.sizes());
+  const int64_t B = parent_.size(0), N = parent_.size(1);
+  const Tensor parent = ints(parent_, at::kInt, {B, N}, parent_, "parent");
+  const optional<Tensor> nodes = ints(nodes_, at::kInt, {B}, parent, "nodes"), pos0 = ints(pos0_, at::kInt, {B}, parent, "pos0");
   const c10::DeviceGuard guard(parent.device());
   Tensor see = at::empty({B, N}, parent.options().dtype(at::kLong)), pos = at::empty({B, N}, parent.options());
   rc_ok(rt_draft_tree(parent.data_ptr<int>(), ptr<int>(nodes), ptr<int>(pos0), (int)B, (int)N, see.data_ptr<int64_t>(), pos.data_ptr<int>(),
                       stream()), "draft_tree");
-  return {see, pos};
+  return {parent, see, pos};
 }
 
-void tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& kv_len, const optional<Tensor>& kv_start,
-                    const Tensor& see, Tensor out, int64_t Hq, int64_t window, double scale) {
+Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& kv_len_, const optional<Tensor>& kv_start_,
+                      const Tensor& see, const optional<Tensor>& out_, int64_t Hq, int64_t window, const optional<double>& scale_) {
   act(qkv, "tree_attention qkv");
-  TORCH_CHECK(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && qkv.stride(1) == 1 && out.dim() == 2 && out.stride(1) == 1,
-              "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim], out [rows nodes, columns]");
+  TORCH_CHECK_VALUE(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && (qkv.stride(1) == 1 || qkv.size(0) == 0),
+                    "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim] expected, got ", qkv.sizes(), ", ", kc.sizes());
   const int64_t B = kc.size(0), Hkv = kc.size(1), Smax = kc.size(2), D = kc.size(3), N = see.size(1);
+  TORCH_CHECK_VALUE(kc.scalar_type() == qkv.scalar_type(), "caches of ", kc.scalar_type(), " under queries of ", qkv.scalar_type(),
+                    ": an fp8 cache is read by decode_step_attention only");
   whole(kc, qkv.scalar_type(), kc.sizes(), qkv, "tree_attention k_cache");
   whole(vc, qkv.scalar_type(), kc.sizes(), qkv, "tree_attention v_cache");
-  whole(kv_len, at::kInt, {B}, qkv, "tree_attention kv_len");
   whole(see, at::kLong, {B, N}, qkv, "tree_attention tree");
-  if (has(kv_start)) whole(*kv_start, at::kInt, {B}, qkv, "tree_attention kv_start");
-  TORCH_CHECK(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && qkv.size(0) == B * N && qkv.size(1) >= (Hq + 2 * Hkv) * D, "tree_attention: qkv shape");
-  on(out, qkv, "tree_attention out");
-  TORCH_CHECK(out.scalar_type() == qkv.scalar_type() && out.size(0) == B * N && out.size(1) == Hq * D, "tree_attention: out shape");
-  TORCH_CHECK(Smax * D < (1L << 30) && window >= 0 && window < (1L << 30) && scale > 0, "tree_attention: sizes");
+  const Tensor kv_len = ints(kv_len_, at::kInt, {B}, qkv, "kv_len");
+  const optional<Tensor> kv_start = ints(kv_start_, at::kInt, {B}, qkv, "kv_start");
+  TORCH_CHECK_VALUE(Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && qkv.size(0) == B * N && qkv.size(1) >= (Hq + 2 * Hkv) * D, "tree_attention: ", Hq,
+                    " heads over ", Hkv, " of ", D, " and ", B, " rows of ", N, " nodes do not fit qkv ", qkv.sizes());
+  const double scale = scale_.has_value() ? *scale_ : 1 / std::sqrt((double)D);
+  TORCH_CHECK_VALUE(window >= 0 && scale > 0 && std::isfinite(scale), "tree_attention: window ", window, ", scale ", scale);
+  TORCH_CHECK_VALUE(D <= 512 && Smax * D < (1L << 30) && window < (1L << 30) && Hq < 65536 && B < 65536, "tree_attention: sizes");
   const c10::DeviceGuard guard(qkv.device());
+  const Tensor out = has(out_) ? *out_ : at::empty({B * N, Hq * D}, qkv.options());
+  on(out, qkv, "tree_attention out");
+  TORCH_CHECK_VALUE(out.scalar_type() == qkv.scalar_type() && out.dim() == 2 && out.size(0) == B * N && out.size(1) == Hq * D &&
+                        (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax) : 0;
   // matrix instructions want rows at 16 bytes (the output at 8): others are copied
@@ -85,32 +105,32 @@ void tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const
                           ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
                           (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, stream()), "tree_attention");
   if (!o.is_same(out)) out.copy_(o);
+  return out;
 }
 
-std::vector<Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens, const Tensor& choice,
-                                const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len) {
+std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens_, const Tensor& choice_,
+                                               const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len_) {
   act(kc, "tree_accept k_cache");
-  TORCH_CHECK(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
+  TORCH_CHECK_VALUE(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
               "tree_accept: caches [layers, rows, heads, slots, dim] and rows of every layer (256 at most)");
   const int64_t L = kc.size(0), B = kc.size(1), Hkv = kc.size(2), Smax = kc.size(3), D = kc.size(4), N = see.size(1);
   on(vc, kc, "tree_accept v_cache");
-  TORCH_CHECK(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
+  TORCH_CHECK_VALUE(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
               "tree_accept: caches of one type and layout, contiguous in each layer");
-  whole(kv_len, at::kInt, {B}, kc, "tree_accept kv_len");
+  const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
   whole(see, at::kLong, {B, N}, kc, "tree_accept tree");
-  whole(tokens, at::kLong, {B, N}, kc, "tree_accept tokens");
-  whole(choice, at::kLong, {B, N}, kc, "tree_accept choice");
+  const Tensor tokens = ints(tokens_, at::kLong, {B, N}, kc, "tokens"), choice = ints(choice_, at::kLong, {B, N}, kc, "choice");
   std::vector<const void*> at;
   for (const Tensor& x : drafts) {
     on(x, kc, "tree_accept drafts");
-    TORCH_CHECK(x.scalar_type() == kc.scalar_type() && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
+    TORCH_CHECK_VALUE(x.scalar_type() == kc.scalar_type() && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
                     x.stride(0) == drafts[0].stride(0) && x.size(0) == B * N && x.size(1) % D == 0 && x.size(1) / D > 2 * Hkv,
                 "tree_accept: drafts [rows nodes, (heads + 2 key heads) dim] of the caches' type, alike in every layer");
     at.push_back(x.data_ptr());
   }
   const int64_t Hq = drafts[0].size(1) / D - 2 * Hkv;
-  TORCH_CHECK(N * Hkv * D < (1L << 30), "tree_accept: sizes");
+  TORCH_CHECK_VALUE(N * Hkv * D < (1L << 30), "tree_accept: sizes");
   const c10::DeviceGuard guard(kc.device());
   Tensor count = at::empty({B}, parent.options()), path = at::empty({B, N}, parent.options()), next = at::empty({B}, tokens.options());
   rc_ok(rt_tree_accept(parent.data_ptr<int>(), see.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), choice.data_ptr<int64_t>(),
@@ -120,16 +140,8 @@ std::vector<Tensor> tree_accept(const Tensor& parent, const Tensor& see, const T
   return {count, path, next};
 }
 
-void logit_rows(const Tensor& logits, const optional<Tensor>& targets, int64_t top) {
-  act(logits, "alternatives logits");
-  TORCH_CHECK(logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1) && logits.size(1) < (1L << 30), "alternatives: logits [tokens, vocabulary]");
-  TORCH_CHECK(top >= 1 && top <= 32 && top <= logits.size(1), "alternatives: 1 to 32 alternatives of the vocabulary");
-  if (has(targets)) whole(*targets, at::kLong, {logits.size(0)}, logits, "alternatives targets");
-}
-
 // -> logp, entropy, alternatives' log-probabilities, their ids, and what the gradient needs of each row
 std::vector<Tensor> alternatives(const Tensor& logits, const optional<Tensor>& targets, double c, int64_t top, bool need_stats) {
-  logit_rows(logits, targets, top);
   const int64_t T = logits.size(0), V = logits.size(1);
   const c10::DeviceGuard guard(logits.device());
   const auto f = logits.options().dtype(at::kFloat);
@@ -137,26 +149,57 @@ std::vector<Tensor> alternatives(const Tensor& logits, const optional<Tensor>& t
   Tensor ids = at::empty({T, top}, logits.options().dtype(at::kLong));
   rc_ok(rt_alternatives(logits.scalar_type() == at::kFloat, logits.data_ptr(), logits.stride(0), ptr<int64_t>(targets), (float)c, T, (int)V,
                         (int)top, logp.data_ptr<float>(), ent.data_ptr<float>(), lp.data_ptr<float>(), ids.data_ptr<int64_t>(),
-                        need_stats ? stats.data_ptr<float>() : nullptr, stream()), "alternatives");
+                        need_stats ? stats.data_ptr<float>() : nullptr, stream()), "token_alternatives");
   return {logp, ent, lp, ids, stats};
 }
 
-Tensor alternatives_bwd(const Tensor& logits, const optional<Tensor>& targets, double c, const Tensor& ids, const Tensor& stats,
-                        const optional<Tensor>& g_lp, const optional<Tensor>& g_ent, const optional<Tensor>& g_top) {
-  TORCH_CHECK(ids.dim() == 2, "alternatives_bwd: ids");
-  const int64_t T = logits.size(0), V = logits.size(1), top = ids.size(1);
-  logit_rows(logits, targets, top);
-  whole(ids, at::kLong, {T, top}, logits, "alternatives_bwd ids");
-  whole(stats, at::kFloat, {T, 3}, logits, "alternatives_bwd stats");
-  for (const auto* g : {&g_lp, &g_ent})
-    if (has(*g)) whole(**g, at::kFloat, {T}, logits, "alternatives_bwd gradients");
-  if (has(g_top)) whole(*g_top, at::kFloat, {T, top}, logits, "alternatives_bwd gradients");
-  const c10::DeviceGuard guard(logits.device());
-  Tensor d = at::empty({T, V}, logits.options());
-  rc_ok(rt_alternatives_bwd(logits.scalar_type() == at::kFloat, logits.data_ptr(), logits.stride(0), ptr<int64_t>(targets), (float)c, T, (int)V,
-                            (int)top, ids.data_ptr<int64_t>(), stats.data_ptr<float>(), ptr<float>(g_lp), ptr<float>(g_ent),
-                            ptr<float>(g_top), d.data_ptr(), d.stride(0), stream()), "alternatives_bwd");
-  return d;
+struct AlternativesFn : torch::autograd::Function<AlternativesFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& targets, double c,
+                                                int64_t top) {
+    auto r = alternatives(logits, targets.defined() ? optional<Tensor>(targets) : c10::nullopt, c, top, true);
+    ctx->save_for_backward({logits, targets, r[3], r[4]});
+    ctx->saved_data["c"] = c;
+    ctx->mark_non_differentiable({r[3]});
+    ctx->set_materialize_grads(false);
+    r.pop_back();
+    return r;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor logits = saved[0], targets = saved[1], ids = saved[2], stats = saved[3];
+    const int64_t T = logits.size(0), V = logits.size(1);
+    for (int i = 0; i < 3; ++i) {
+      TORCH_CHECK(!grads[i].defined() || !grads[i].requires_grad() || !at::GradMode::is_enabled(), "token_alternatives has no second derivative");
+      if (grads[i].defined()) grads[i] = grads[i].to(at::kFloat).contiguous();
+    }
+    auto g = [&](int i) { return grads[i].defined() ? grads[i].data_ptr<float>() : nullptr; };
+    const c10::DeviceGuard guard(logits.device());
+    Tensor d = at::empty({T, V}, logits.options());
+    rc_ok(rt_alternatives_bwd(logits.scalar_type() == at::kFloat, logits.data_ptr(), logits.stride(0),
+                              targets.defined() ? targets.data_ptr<int64_t>() : nullptr, (float)ctx->saved_data["c"].toDouble(), T, (int)V,
+                              (int)ids.size(1), ids.data_ptr<int64_t>(), stats.data_ptr<float>(), g(0), g(1), g(2), d.data_ptr(), d.stride(0),
+                              stream()), "token_alternatives backward");
+    return {d, Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> token_alternatives(const Tensor& logits, const optional<Tensor>& targets, int64_t top, double c) {
+  act(logits, "logits");
+  TORCH_CHECK_VALUE(logits.dim() == 2 && top >= 1 && top <= 32 && top <= logits.size(1) && logits.size(1) < (1L << 30),
+                    "1 to 32 alternatives of logits [tokens, vocabulary] expected: ", top, " of ", logits.sizes());
+  TORCH_CHECK_VALUE(c > 0 && std::isfinite((float)c), "inverse temperature ", c);
+  const Tensor x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
+  Tensor t;
+  if (has(targets)) {
+    on(*targets, logits, "targets");
+    TORCH_CHECK_VALUE(targets->dim() == 1 && targets->size(0) == logits.size(0) && at::isIntegralType(targets->scalar_type(), false),
+                      "targets: ", logits.size(0), " whole numbers expected, got ", targets->scalar_type(), " ", targets->sizes());
+    t = targets->to(at::kLong).contiguous();
+  }
+  auto r = at::GradMode::is_enabled() && x.requires_grad() ? AlternativesFn::apply(x, t, c, top)
+                                                            : alternatives(x, t.defined() ? optional<Tensor>(t) : c10::nullopt, c, top, false);
+  return {r[0], r[1], r[2], r[3]};
 }
 
 }  // namespace
@@ -165,6 +208,5 @@ void bind_drafts(py::module_& m) {
   m.def("draft_tree", &draft_tree, "ancestors and positions of drafted tokens");
   m.def("tree_attention", &tree_attention, "attention of drafted tokens over the cache and their ancestors");
   m.def("tree_accept", &tree_accept, "the agreed path of a tree, appended to the caches");
-  m.def("alternatives", &alternatives, "log-probabilities of tokens, entropy and the best alternatives");
-  m.def("alternatives_bwd", &alternatives_bwd, "gradient of alternatives");
+  m.def("token_alternatives", &token_alternatives, "log-probabilities of tokens, entropy and the best alternatives (differentiable)");
 }

@@ -43,13 +43,14 @@ def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0:
     """The plan of drafted trees: ``parent`` int32 [rows, nodes <= 64] holds an earlier node of the row for each (anything else: none, a tree of its
     own), ``nodes`` int32 [rows] how many of a row's are nodes (0: the row idles; default all), ``pos0`` int32 [rows] the position
     of node 0 (default 0)."""
+    if on_gpu(parent):
+        return DraftTree(*native().draft_tree(parent, nodes, pos0))
     if parent.dim() != 2 or not 1 <= parent.shape[1] <= MAX_NODES:
         raise ValueError(f"parent: [rows, 1 .. {MAX_NODES} nodes] expected, got {tuple(parent.shape)}")
     parent = _ints(parent, "parent", parent.shape, parent)
     nodes = None if nodes is None else _ints(nodes, "nodes", parent.shape[:1], parent)
     pos0 = None if pos0 is None else _ints(pos0, "pos0", parent.shape[:1], parent)
-    see, pos = native().draft_tree(parent, nodes, pos0) if on_gpu(parent) else ref.draft_tree(parent, nodes, pos0)
-    return DraftTree(parent, see, pos)
+    return DraftTree(parent, *ref.draft_tree(parent, nodes, pos0))
 
 
 def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, tree: DraftTree, Hq: int,
@@ -59,6 +60,8 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
     key; with ``window`` only those less than ``window`` positions before it. Nothing is appended to the caches; rows that are not
     nodes come out as zeros. What other nodes hold, NaN among it, does not reach a node."""
+    if on_gpu(qkv):
+        return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     B, Hkv, Smax, D = k_cache.shape
@@ -74,13 +77,8 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"window {window}, scale {scale}")
     kv_len = _ints(kv_len, "kv_len", (B,), qkv)
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
-    if out is None:
-        out = torch.empty(B * N, Hq * D, dtype=qkv.dtype, device=qkv.device)
-    if on_gpu(qkv):
-        native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale)
-    else:
-        out.copy_(ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale))
-    return out
+    o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale)
+    return o if out is None else out.copy_(o)
 
 
 def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, drafts: List[torch.Tensor], k_cache: torch.Tensor,
@@ -90,6 +88,8 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
     on with the child whose token is the choice (the first of equal ones). Keys and values of its nodes go from ``drafts``
     (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
     itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out."""
+    if on_gpu(k_cache):
+        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len)
     if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     L, B, Hkv, Smax, D = k_cache.shape
@@ -101,6 +101,4 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
                                or x.shape[1] % D or x.shape[1] <= 2 * Hkv * D for x in drafts):
         raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")
     kv_len = _ints(kv_len, "kv_len", (B,), k_cache)
-    if on_gpu(k_cache):
-        return tuple(native().tree_accept(tree.parent, tree.see, tokens.contiguous(), choice.contiguous(), drafts, k_cache, v_cache, kv_len))
     return ref.tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len)

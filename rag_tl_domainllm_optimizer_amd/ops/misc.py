@@ -150,45 +150,20 @@ def token_logprobs(logits: torch.Tensor, targets, inv_temp: float = 1.0):
     return lp, ent
 
 
-class _AlternativesFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets, top, inv_temp):
-        lp, ent, top_lp, ids, stats = native().alternatives(logits, targets, inv_temp, top, True)
-        ctx.save_for_backward(logits, targets, ids, stats)
-        ctx.inv_temp = inv_temp
-        ctx.mark_non_differentiable(ids)
-        ctx.set_materialize_grads(False)
-        return lp, ent, top_lp, ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        logits, targets, ids, stats = ctx.saved_tensors
-        g = [None if x is None else x.float().contiguous() for x in grads[:3]]
-        return native().alternatives_bwd(logits, targets, ctx.inv_temp, ids, stats, *g), None, None, None
-
-
 def token_alternatives(logits: torch.Tensor, targets, top: int, inv_temp: float = 1.0):
     """:func:`token_logprobs` with the best alternatives: logits [T, V] (bf16 or fp32; rows may be strided) -> (log p(target) [T], entropy [T], the
     log-probabilities of the ``top`` (1 to 32) most likely tokens, best first [T, top], their ids int64 [T, top]) of softmax(logits * inv_temp),
     all but the ids differentiable. Targets below 0, or None, have log-probability 0; a target from V on has NaN on a GPU. Equally likely tokens go by their id and a NaN logit counts as the least likely; a row of -inf alone has log-probabilities
     of -inf, entropy 0 and no gradient."""
+    if on_gpu(logits):
+        return native().token_alternatives(logits, targets, top, inv_temp)
     if logits.dim() != 2 or not 1 <= top <= min(32, logits.shape[1]):
         raise ValueError(f"1 to 32 alternatives of logits [tokens, vocabulary] expected: {top} of {tuple(logits.shape)}")
     if not (inv_temp > 0 and np.isfinite(inv_temp)):
         raise ValueError(f"inverse temperature {inv_temp}")
     if targets is not None and (tuple(targets.shape) != tuple(logits.shape[:1]) or targets.is_floating_point() or targets.device != logits.device):
         raise ValueError(f"targets: {logits.shape[0]} whole numbers on {logits.device} expected")
-    if not on_gpu(logits):
-        return ref.alternatives(logits, targets, top, inv_temp)
-    if logits.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"logits of {logits.dtype}: bf16 or fp32 expected")
-    if logits.stride(1) != 1 and logits.shape[1] > 1:
-        logits = logits.contiguous()
-    targets = None if targets is None else targets.long().contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _AlternativesFn.apply(logits, targets, top, float(inv_temp))
-    return tuple(native().alternatives(logits, targets, float(inv_temp), top, False)[:4])
+    return ref.alternatives(logits, targets, top, inv_temp)
 
 
 # --------------------------------------------------------------------------------- sampler
