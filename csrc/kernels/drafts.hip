@@ -5,6 +5,7 @@
 #include "rt_paged.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace rt {
 namespace drafts {
@@ -52,6 +53,7 @@ struct TreeArgs {
   void* o; long ldo;
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
+  int sorted;
   float* part; int S;                   // [S, B, Hkv, N Hq / Hkv, D + 2] partials (o | m | l) of at most S shares of a row's keys
 };
 
@@ -148,6 +150,20 @@ __device__ __forceinline__ uint64_t near_nodes(uint64_t see, int window) {
   return see;
 }
 
+// the row that has q longer ones before it (64 rows at most, one a lane): long rows first where a CU takes several
+__device__ __forceinline__ int longest(const TreeArgs& a, int q, int lane) {
+  const int len = lane < a.B ? min(max(a.kv_len[lane], 0), a.Smax) : -1;
+  int before = 0;
+  for (int j = 0; j < a.B; ++j) {
+    const int other = __builtin_amdgcn_readlane(len, j);
+    before += other > len || (other == len && j < lane);
+  }
+  return __builtin_ctzll(__ballot(lane < a.B && before == q));
+}
+
+// one v_maximum3_f32 for two of these; fmaxf has each operand made canonical first. A NaN stays one.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 template <int D, int RT, int WR, int WK, int KT>
 __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
@@ -156,7 +172,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   __shared__ unsigned bad[2];  // nodes whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   const int s = blockIdx.x % a.S, pair = blockIdx.x / a.S % (a.B * a.Hkv), rb = blockIdx.x / a.S / (a.B * a.Hkv);
-  const int b = pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
+  const int b = a.sorted ? longest(a, pair / a.Hkv, lane) : pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
   const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
   const uint64_t live = __ballot(see != 0);
   const int n = live ? 64 - __builtin_clzll(live) : 0, M = n * G;
@@ -189,31 +205,54 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
       for (int c = 0; c < DT; ++c) o[u][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const long head = ((long)b * a.Hkv + gh) * a.Smax * D;
-    auto stage = [&](int tile, int buf) {
-      const bool own = tile == ct.tiles - 1;
-      const bf16_t* const kb = own ? x + (long)(a.Hq + gh) * D : (const bf16_t*)a.kc + head;
-      const bf16_t* const vb = own ? x + (long)(a.Hq + a.Hkv + gh) * D : (const bf16_t*)a.vc + head;
-      const int first = own ? 0 : ct.lo + tile * SK, last = (own ? n : ct.len) - 1, pitch = own ? (int)a.ldq * 2 : D * 2;
+    const bf16_t* const kc = (const bf16_t*)a.kc + head + (long)ct.lo * D;
+    const bf16_t* const vc = (const bf16_t*)a.vc + head + (long)ct.lo * D;
+    const int full = (ct.len - ct.lo) / SK;  // stages of SK keys
+    constexpr int NJ = KB / 1024 / NW;       // this wave's loads of the keys' (values') image
+    uint32_t off[2 * NJ];
+    int key_of[NJ];
 #pragma unroll
-      for (int j = 0; j < 2 * KB / 1024 / NW; ++j) {
-        const bool v = j >= KB / 1024 / NW;
-        const int at = (v ? j - KB / 1024 / NW : j) * NW + wid, e = at * 64 + lane, key = e / NC;
-        const int c = v ? paged::vv_chunk<D>(key, e % NC) : paged::kq_chunk<D>(key, e % NC);
-        // keys behind the last one repeat it: they are masked, and what lies there is nobody's
-        paged::lds_dma16(v ? vb : kb, (uint32_t)(min(first + key, last) * pitch + 16 * c), smem + (2 * buf + v) * KB + at * 1024);
+    for (int j = 0; j < NJ; ++j) {
+      const int e = (j * NW + wid) * 64 + lane, key = e / NC;
+      key_of[j] = key;
+      off[j] = key * D * 2 + 16 * paged::kq_chunk<D>(key, e % NC);
+      off[NJ + j] = key * D * 2 + 16 * paged::vv_chunk<D>(key, e % NC);
+    }
+    auto stage = [&](int tile, int buf) {
+      char* const dst = smem + 2 * buf * KB + wid * 1024;
+      if (tile < full) {
+        const long at = (long)tile * SK * D;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          paged::lds_dma16(kc + at, off[j], dst + j * NW * 1024);
+          paged::lds_dma16(vc + at, off[NJ + j], dst + KB + j * NW * 1024);
+        }
+        return;
+      }
+      // keys behind the last one repeat it: they are masked, and what lies there is nobody's
+      const bool own = tile == ct.tiles - 1;
+      const bf16_t* const kb = own ? x + (long)(a.Hq + gh) * D : kc + (long)tile * SK * D;
+      const bf16_t* const vb = own ? x + (long)(a.Hq + a.Hkv + gh) * D : vc + (long)tile * SK * D;
+      const int last = own ? n - 1 : ct.len - ct.lo - tile * SK - 1, pitch = own ? (int)a.ldq * 2 : D * 2;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int key = min(key_of[j], last) * pitch;
+        paged::lds_dma16(kb, (uint32_t)(key + (off[j] & (2 * D - 1))), dst + j * NW * 1024);
+        paged::lds_dma16(vb, (uint32_t)(key + (off[NJ + j] & (2 * D - 1))), dst + KB + j * NW * 1024);
       }
     };
     if (tid < 2) bad[tid] = 0;
     stage(t0, 0);
     int cur = 0;
-    for (int t = t0; t < t1; ++t, cur ^= 1) {
+    // one stage; MODE 0: every row sees all of its keys, 1: some keys of the context are not seen, 2: the nodes' own keys
+    auto turn = [&](auto mode, int t) {
+      constexpr int MODE = decltype(mode)::value;
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
-      asm volatile("s_barrier" ::: "memory");           // ... by every wave; the other buffer is free
-      if (t + 1 < t1) stage(t + 1, cur ^ 1);
-      const bool own = t == ct.tiles - 1;
+      asm volatile("s_barrier" ::: "memory");                      // ... by every wave; the other buffer is free
+      if (MODE != 2 && t + 1 < t1) stage(t + 1, cur ^ 1);
       char* const Ks = smem + 2 * cur * KB + wk * KT * D * 2;
       char* const Vs = smem + (2 * cur + 1) * KB + wk * KT * D * 2;
-      if (own) {
+      if constexpr (MODE == 2) {
         // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
         // product and are added below for the rows that see them
         char* const img = smem + (2 * cur + 1) * KB;
@@ -230,7 +269,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         }
         __syncthreads();
       }
-      if (row0 >= M) continue;
+      cur ^= 1;
+      if (row0 >= M) return;
       f32x4 st[KS][RT];
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -246,7 +286,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
           for (int u = 0; u < RT; ++u) st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][d], st[k][u], 0, 0, 0);
         }
       const int key0 = wk * KT + 4 * g;  // of the stage: this lane's keys are key0 + 16 k + e
-      if (own) {
+      if constexpr (MODE == 2) {
 #pragma unroll
         for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -256,30 +296,48 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
             for (int e = 0; e < 4; ++e)
               if (!(bits >> e & 1)) st[k][u][e] = -INFINITY;
           }
-      } else {
-        const int first = ct.lo + t * SK;
-        if (first + SK > ct.len || (a.window && first < ct.len + NODES - a.window)) {
+      }
+      if constexpr (MODE == 1) {
+        const int first = ct.lo + t * SK + key0;
 #pragma unroll
-          for (int u = 0; u < RT; ++u)
+        for (int u = 0; u < RT; ++u)
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+          for (int k = 0; k < KS; ++k)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = first + key0 + 16 * k + e;
-                if (key >= ct.len || key < from[u]) st[k][u][e] = -INFINITY;
-              }
-        }
+            for (int e = 0; e < 4; ++e) {
+              const int key = first + 16 * k + e;
+              if (key >= ct.len || key < from[u]) st[k][u][e] = -INFINITY;
+            }
       }
       float alpha[RT];
+      bool grown = false;
+      float mn[RT];
 #pragma unroll
       for (int u = 0; u < RT; ++u) {
-        float mx = -INFINITY;
+        float mx = st[0][u][0];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) mx = fmaxf(mx, fmaxf(fmaxf(st[k][u][0], st[k][u][1]), fmaxf(st[k][u][2], st[k][u][3])));
-        const float mn = fmaxf(m[u], over_groups(mx, [](float p, float q) { return fmaxf(p, q); }));
-        const float mz = (mn == -INFINITY ? 0.f : mn) * a.scale;  // a row may see nothing of its first stages
-        alpha[u] = paged::fexp2(m[u] * a.scale - mz);
-        m[u] = mn;
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx = larger(mx, st[k][u][e]);
+        mn[u] = larger(m[u], over_groups(mx, [](float p, float q) { return larger(p, q); }));
+        grown = grown || !((mn[u] - m[u]) * a.scale <= 8.f || mn[u] == m[u]);
+      }
+      // the maximum that p is taken from follows the rows' own only by steps: up to 2^8 instead of 1 costs nothing in fp32, and o is seldom
+      // multiplied
+      if (__any(grown)) {
+#pragma unroll
+        for (int u = 0; u < RT; ++u) {
+          const float mz = (mn[u] == -INFINITY ? 0.f : mn[u]) * a.scale;  // a row may see nothing of its first stages
+          alpha[u] = paged::fexp2(m[u] * a.scale - mz);
+          m[u] = mn[u];
+          l[u] *= alpha[u];
+#pragma unroll
+          for (int c = 0; c < DT; ++c) o[u][c] *= alpha[u];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < RT; ++u) {
+        const float mz = (m[u] == -INFINITY ? 0.f : m[u]) * a.scale;
         float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -289,16 +347,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
             st[k][u][e] = p;
             sum += p;
           }
-        l[u] = l[u] * alpha[u] + sum;  // of this lane's keys; the four lanes are added at the end
-      }
-      bool grown = false;
-#pragma unroll
-      for (int u = 0; u < RT; ++u) grown = grown || alpha[u] != 1.f;
-      if (__any(grown)) {
-#pragma unroll
-        for (int u = 0; u < RT; ++u)
-#pragma unroll
-          for (int c = 0; c < DT; ++c) o[u][c] *= alpha[u];
+        l[u] += sum;  // of this lane's keys; the four lanes are added at the end
       }
       bf16x8 pf[KT / 32][RT];
 #pragma unroll
@@ -334,7 +383,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
           }
         }
       }
-      if (own) {
+      if constexpr (MODE == 2) {
         const uint64_t ill = ((uint64_t)bad[1] << 32 | bad[0]) & (KT == 64 ? ~0ull : 0xffffffffull << (wk * KT));
         for (uint64_t w = ill; w; w &= w - 1) {
           const int node = __builtin_ctzll(w);
@@ -351,7 +400,13 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
                 }
         }
       }
-    }
+    };
+    int t = t0;
+    if (a.window)  // stages that the last nodes do not see all of
+      for (; t < min(t1, ct.tiles - 1) && ct.lo + t * SK < ct.len + NODES - a.window; ++t) turn(std::integral_constant<int, 1>(), t);
+    for (; t < min(t1, full); ++t) turn(std::integral_constant<int, 0>(), t);
+    for (; t < min(t1, ct.tiles - 1); ++t) turn(std::integral_constant<int, 1>(), t);
+    if (t < t1) turn(std::integral_constant<int, 2>(), t);
 #pragma unroll
     for (int u = 0; u < RT; ++u) l[u] = over_groups(l[u], [](float p, float q) { return p + q; });
     if constexpr (WK > 1) {  // the keys' shares, joined in order
@@ -548,7 +603,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
                                  int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, part, S};
+  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, part, S};
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
     if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
@@ -559,6 +614,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   if (f32 || (D != 64 && D != 128) || (S > 1 && !part)) return -1;
   a.scale = scale * 1.4426950408889634f;
   const int rows = N * (Hq / Hkv);
+  a.sorted = B > 1 && B <= 64 && (long)B * Hkv * S * ((rows + 255) / 256) > num_cus();
   const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
