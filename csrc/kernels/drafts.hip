@@ -188,7 +188,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     int from[RT];  // first key of the context that the row sees
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      const int r = min(row0 + 16 * u + r16, M - 1), node = r / G;
+      const int r = min(row0 + 16 * u + r16, a.N * G - 1), node = r / G;
       const bf16_t* const q = x + (long)node * a.ldq + (long)(gh * G + r % G) * D + 8 * g;
 #pragma unroll
       for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
@@ -472,34 +472,78 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   }
 }
 
-// the parts of rows that were cut, one wave a (node, head)
-template <int D>
+// The parts of rows that were cut: WAVES waves a (node, head), eight parts each under way at once. The first eight are read before the
+// lengths that say how many there are (what lies in the others is in the buffer, and not used): one trip to memory instead of two.
+template <int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
-  const int lane = threadIdx.x & 63, G = a.Hq / a.Hkv, per = a.N * G;
-  const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6), pair = w / per;
-  const int r = (int)(w % per);
-  if (pair >= (long)a.B * a.Hkv) return;
-  const int b = (int)(pair / a.Hkv), gh = (int)(pair % a.Hkv);
-  if (!a.see[(long)b * a.N + r / G]) return;
-  const Cut ct = cut(a, b, SK);
-  if (ct.parts == 1) return;
+  constexpr int W = D / 64;
+  __shared__ float sh[4][64 * W + 2];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w = wid % WAVES, G = a.Hq / a.Hkv, per = a.N * G;
+  const long at = (long)blockIdx.x * (4 / WAVES) + wid / WAVES, pair = min(at / per, (long)a.B * a.Hkv - 1);
+  const int r = (int)(at % per), b = (int)(pair / a.Hkv), gh = (int)(pair % a.Hkv);
   const long step = (long)a.B * a.Hkv * per * (D + 2);
   const float* const p = a.part + (pair * per + r) * (D + 2);
-  float m = -INFINITY, l = 0.f, o[D / 64];
+  float m = -INFINITY, l = 0.f, o[W];
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) o[i] = 0.f;
-  for (int s = 0; s < ct.parts; ++s) {
-    const float* const q = p + s * step;
-    const float ms = q[D], mn = fmaxf(m, ms), mz = mn == -INFINITY ? 0.f : mn;
-    const float x0 = paged::fexp2(m - mz), x1 = paged::fexp2(ms - mz);
-    m = mn;
-    l = l * x0 + q[D + 1] * x1;
+  for (int i = 0; i < W; ++i) o[i] = 0.f;
+  int parts = a.S;
+  for (int s0 = 8 * w; s0 < parts; s0 += 8 * WAVES) {
+    float pm[8], pl[8], po[8][W];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] = o[i] * x0 + q[D / 64 * lane + i] * x1;
+    for (int k = 0; k < 8; ++k) {
+      const float* const q = p + min(s0 + k, a.S - 1) * step;
+      pm[k] = q[D];
+      pl[k] = q[D + 1];
+#pragma unroll
+      for (int i = 0; i < W; ++i) po[k][i] = q[W * lane + i];
+    }
+    parts = cut(a, b, SK).parts;
+    float mx = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (s0 + k >= parts) pm[k] = -INFINITY;
+      mx = larger(mx, pm[k]);
+    }
+    const float mz = mx == -INFINITY ? 0.f : mx, old = paged::fexp2(m - mz);
+    m = mx;
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] *= old;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float x = paged::fexp2(pm[k] - mz);
+      if (s0 + k >= parts) continue;
+      l = fmaf(pl[k], x, l);
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = fmaf(po[k][i], x, o[i]);
+    }
   }
-  bf16_t* const out = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + D / 64 * lane;
-  if constexpr (D == 128) *(uint32_t*)out = pack2bf(o[0] / l, o[1] / l);
-  else out[0] = f2bf(o[0] / l);
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) sh[wid][W * lane + i] = o[i];
+    if (lane == 0) { sh[wid][64 * W] = m; sh[wid][64 * W + 1] = l; }
+    __syncthreads();
+    if (w) return;
+    float mx = m;
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) mx = larger(mx, sh[wid + k][64 * W]);
+    const float mz = mx == -INFINITY ? 0.f : mx, old = paged::fexp2(m - mz);
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < W; ++i) o[i] *= old;
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) {
+      const float x = paged::fexp2(sh[wid + k][64 * W] - mz);
+      l = fmaf(sh[wid + k][64 * W + 1], x, l);
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[i] = fmaf(sh[wid + k][W * lane + i], x, o[i]);
+    }
+  }
+  if (at / per > pair || parts == 1 || !a.see[(long)b * a.N + r / G]) return;
+  bf16_t* const out = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + W * lane;
+  const float inv = 1.f / l;
+  if constexpr (W == 2) *(uint32_t*)out = pack2bf(o[0] * inv, o[1] * inv);
+  else out[0] = f2bf(o[0] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -591,6 +635,12 @@ static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
   return 0;
 }
 
+template <int D>
+static void launch_join(const TreeArgs& a, long rows, hipStream_t stream) {
+  if (a.S <= 8) hipLaunchKernelGGL((tree_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, 64);
+  else hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, 64);
+}
+
 // parts that a row's keys may be cut in: the partials that rt_tree_attention wants. 0: sizes without matrix instructions
 extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax) {
   if ((D != 64 && D != 128) || B == 0) return 0;
@@ -618,9 +668,9 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
-    const dim3 grid((unsigned)(((long)B * Hkv * rows + 3) / 4));
-    if (D == 128) hipLaunchKernelGGL(tree_join_kernel<128>, grid, dim3(256), 0, stream, a, 64);
-    else hipLaunchKernelGGL(tree_join_kernel<64>, grid, dim3(256), 0, stream, a, 64);
+    const long all = (long)B * Hkv * rows;
+    if (D == 128) launch_join<128>(a, all, stream);
+    else launch_join<64>(a, all, stream);
     RT_LAUNCH_CHECK();
   }
   return 0;
