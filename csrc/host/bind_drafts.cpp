@@ -100,7 +100,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   Tensor x = qkv, o = out;
   if (S && !(al(x, 16) && x.stride(0) % 8 == 0 && x.stride(0) < (1L << 24))) x = qkv.narrow(1, 0, (Hq + 2 * Hkv) * D).clone(at::MemoryFormat::Contiguous);
   if (S && !(al(o, 8) && o.stride(0) % 4 == 0)) o = at::empty({B * N, Hq * D}, qkv.options());
-  Tensor part = S > 1 ? at::empty({S * B * Hq * N * (D + 2)}, qkv.options().dtype(at::kFloat)) : Tensor();
+  Tensor part = S > 1 ? at::empty({S * B * Hkv * ((N * (Hq / Hkv) + 15) / 16) * 16 * (D + 2)}, qkv.options().dtype(at::kFloat)) : Tensor();
   rc_ok(rt_tree_attention(x.scalar_type() == at::kFloat, x.data_ptr(), x.stride(0), kc.data_ptr(), vc.data_ptr(), kv_len.data_ptr<int>(),
                           ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
                           (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, stream()), "tree_attention");

@@ -54,7 +54,7 @@ struct TreeArgs {
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
   int sorted;
-  float* part; int S;                   // [S, B, Hkv, N Hq / Hkv, D + 2] partials (o | m | l) of at most S shares of a row's keys
+  float* part; int S;                   // partials of at most S shares of a row's keys (part_of)
 };
 
 template <typename T>
@@ -138,9 +138,15 @@ __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int SK) {
   if (a.window) c.lo = max(c.lo, c.len - a.window + 1);
   c.lo = min(c.lo, c.len);
   c.tiles = (c.len - c.lo + SK - 1) / SK + 1;
-  c.per = max((c.tiles + a.S - 1) / a.S, min(c.tiles, 2));
+  c.per = (c.tiles + a.S - 1) / a.S;
   c.parts = (c.tiles + c.per - 1) / c.per;
   return c;
+}
+
+// a part of a pair's rows: of each 16 of them the accumulators as the lanes hold them [D / 16][64][4], behind all of these (m, l) of each row
+__device__ __forceinline__ int tiles16(const TreeArgs& a) { return (a.N * (a.Hq / a.Hkv) + 15) / 16; }
+__device__ __forceinline__ float* part_of(const TreeArgs& a, int D, int s, long pair) {
+  return a.part + ((long)s * a.B * a.Hkv + pair) * ((long)tiles16(a) * 16 * (D + 2));
 }
 
 // ancestors less than `window` positions before a node: the last ones
@@ -181,6 +187,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   const int t0 = s * ct.per, t1 = min(t0 + ct.per, ct.tiles);
   const int row0 = rb * ROWS + wr * 16 * RT;  // of this wave
   const bf16_t* const x = (const bf16_t*)a.qkv + (long)b * a.N * a.ldq;
+  const long pair_at = (long)b * a.Hkv + gh;
 
   if (rb * ROWS < M) {
     bf16x8 qf[RT][DS];
@@ -410,52 +417,45 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
 #pragma unroll
     for (int u = 0; u < RT; ++u) l[u] = over_groups(l[u], [](float p, float q) { return p + q; });
     if constexpr (WK > 1) {  // the keys' shares, joined in order
-      float* const sh = (float*)smem;
-      for (int k = 1; k < WK; ++k) {
-        __syncthreads();
-        if (wk == k) {
+      float* const sh = (float*)smem + wr * (4 * DT + 2) * 64 + lane;
+      static_assert(WR * (4 * DT + 2) * 256 <= 4 * KB);
 #pragma unroll
-          for (int u = 0; u < RT; ++u) {
-            float* const p = sh + ((wr * RT + u) * (DT * 4 + 2)) * 64 + lane;
-            p[0] = m[u];
-            p[64] = l[u];
+      for (int u = 0; u < RT; ++u)
+        for (int k = 1; k < WK; ++k) {
+          __syncthreads();
+          if (wk == k) {
+            sh[0] = m[u];
+            sh[64] = l[u];
 #pragma unroll
             for (int c = 0; c < DT; ++c)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) p[(2 + 4 * c + e) * 64] = o[u][c][e];
+              for (int e = 0; e < 4; ++e) sh[(2 + 4 * c + e) * 64] = o[u][c][e];
           }
-        }
-        __syncthreads();
-        if (wk == 0) {
-#pragma unroll
-          for (int u = 0; u < RT; ++u) {
-            const float* const p = sh + ((wr * RT + u) * (DT * 4 + 2)) * 64 + lane;
-            const float mn = fmaxf(m[u], p[0]), mz = (mn == -INFINITY ? 0.f : mn) * a.scale;
-            const float x0 = paged::fexp2(m[u] * a.scale - mz), x1 = paged::fexp2(p[0] * a.scale - mz);
+          __syncthreads();
+          if (wk == 0) {
+            const float mn = larger(m[u], sh[0]), mz = (mn == -INFINITY ? 0.f : mn) * a.scale;
+            const float x0 = paged::fexp2(m[u] * a.scale - mz), x1 = paged::fexp2(sh[0] * a.scale - mz);
             m[u] = mn;
-            l[u] = l[u] * x0 + p[64] * x1;
+            l[u] = l[u] * x0 + sh[64] * x1;
 #pragma unroll
             for (int c = 0; c < DT; ++c)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) o[u][c][e] = o[u][c][e] * x0 + p[(2 + 4 * c + e) * 64] * x1;
+              for (int e = 0; e < 4; ++e) o[u][c][e] = o[u][c][e] * x0 + sh[(2 + 4 * c + e) * 64] * x1;
           }
         }
-      }
-      if (wk) return;
     }
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
+      if (wk) break;
       const int r = row0 + 16 * u + r16;
-      if (r >= M) continue;
       if (ct.parts > 1) {
-        float* const p = a.part + (((long)s * a.B + b) * a.Hkv + gh) * ((long)a.N * G * (D + 2)) + (long)r * (D + 2);
-        if (g == 0) { p[D] = m[u] * a.scale; p[D + 1] = l[u]; }
+        if (row0 + 16 * u >= M) continue;
+        float* const p = part_of(a, D, s, pair_at);
+        if (g == 0) *(float2*)(p + tiles16(a) * 16 * D + 2 * r) = make_float2(m[u] * a.scale, l[u]);
+        f32x4* const q = (f32x4*)(p + (long)(row0 + 16 * u) * D) + lane;
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          *(float2*)(p + 16 * c + 4 * g) = make_float2(o[u][c][0], o[u][c][1]);
-          *(float2*)(p + 16 * c + 4 * g + 2) = make_float2(o[u][c][2], o[u][c][3]);
-        }
-      } else {
+        for (int c = 0; c < DT; ++c) q[64 * c] = o[u][c];
+      } else if (r < M) {
         const float inv = 1.f / l[u];  // a node sees itself
         bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 4 * g;
 #pragma unroll
@@ -472,78 +472,73 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   }
 }
 
-// The parts of rows that were cut: WAVES waves a (node, head), eight parts each under way at once. The first eight are read before the
-// lengths that say how many there are (what lies in the others is in the buffer, and not used): one trip to memory instead of two.
+// The parts of rows that were cut: WAVES waves for 16 rows' accumulators of 16 columns, eight parts each under way at once. The first
+// eight are read before the lengths that say how many there are (what lies in the others is in the buffer, and not used): one trip to
+// memory instead of two.
 template <int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
-  constexpr int W = D / 64;
-  __shared__ float sh[4][64 * W + 2];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w = wid % WAVES, G = a.Hq / a.Hkv, per = a.N * G;
-  const long at = (long)blockIdx.x * (4 / WAVES) + wid / WAVES, pair = min(at / per, (long)a.B * a.Hkv - 1);
-  const int r = (int)(at % per), b = (int)(pair / a.Hkv), gh = (int)(pair % a.Hkv);
-  const long step = (long)a.B * a.Hkv * per * (D + 2);
-  const float* const p = a.part + (pair * per + r) * (D + 2);
-  float m = -INFINITY, l = 0.f, o[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) o[i] = 0.f;
+  __shared__ float sh[4][6][64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w = wid % WAVES, r16 = lane & 15, g = lane >> 4, G = a.Hq / a.Hkv;
+  const int tiles = tiles16(a);
+  const long all = (long)a.B * a.Hkv * tiles * (D / 16), id = (long)blockIdx.x * (4 / WAVES) + wid / WAVES, at = min(id, all - 1);
+  const int c = (int)(at % (D / 16)), tile = (int)(at / (D / 16) % tiles);
+  const long pair = at / (D / 16) / tiles;
+  const int b = (int)(pair / a.Hkv), gh = (int)(pair % a.Hkv), r = 16 * tile + r16;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
   int parts = a.S;
   for (int s0 = 8 * w; s0 < parts; s0 += 8 * WAVES) {
-    float pm[8], pl[8], po[8][W];
+    float2 ml[8];
+    f32x4 po[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float* const q = p + min(s0 + k, a.S - 1) * step;
-      pm[k] = q[D];
-      pl[k] = q[D + 1];
-#pragma unroll
-      for (int i = 0; i < W; ++i) po[k][i] = q[W * lane + i];
+      const float* const q = part_of(a, D, min(s0 + k, a.S - 1), pair);
+      ml[k] = *(const float2*)(q + tiles * 16 * D + 2 * r);
+      po[k] = ((const f32x4*)(q + 16 * tile * D))[64 * c + lane];
     }
     parts = cut(a, b, SK).parts;
     float mx = m;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (s0 + k >= parts) pm[k] = -INFINITY;
-      mx = larger(mx, pm[k]);
-    }
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < parts) mx = larger(mx, ml[k].x);
     const float mz = mx == -INFINITY ? 0.f : mx, old = paged::fexp2(m - mz);
     m = mx;
     l *= old;
+    o *= old;
 #pragma unroll
-    for (int i = 0; i < W; ++i) o[i] *= old;
+    for (int k = 0; k < 8; ++k)
+      if (s0 + k < parts) {
+        const float x = paged::fexp2(ml[k].x - mz);
+        l = fmaf(ml[k].y, x, l);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float x = paged::fexp2(pm[k] - mz);
-      if (s0 + k >= parts) continue;
-      l = fmaf(pl[k], x, l);
-#pragma unroll
-      for (int i = 0; i < W; ++i) o[i] = fmaf(po[k][i], x, o[i]);
-    }
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(po[k][e], x, o[e]);
+      }
   }
   if constexpr (WAVES > 1) {
+    sh[wid][0][lane] = m;
+    sh[wid][1][lane] = l;
 #pragma unroll
-    for (int i = 0; i < W; ++i) sh[wid][W * lane + i] = o[i];
-    if (lane == 0) { sh[wid][64 * W] = m; sh[wid][64 * W + 1] = l; }
+    for (int e = 0; e < 4; ++e) sh[wid][2 + e][lane] = o[e];
     __syncthreads();
     if (w) return;
     float mx = m;
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) mx = larger(mx, sh[wid + k][64 * W]);
+    for (int k = 1; k < WAVES; ++k) mx = larger(mx, sh[wid + k][0][lane]);
     const float mz = mx == -INFINITY ? 0.f : mx, old = paged::fexp2(m - mz);
     l *= old;
-#pragma unroll
-    for (int i = 0; i < W; ++i) o[i] *= old;
+    o *= old;
 #pragma unroll
     for (int k = 1; k < WAVES; ++k) {
-      const float x = paged::fexp2(sh[wid + k][64 * W] - mz);
-      l = fmaf(sh[wid + k][64 * W + 1], x, l);
+      const float x = paged::fexp2(sh[wid + k][0][lane] - mz);
+      l = fmaf(sh[wid + k][1][lane], x, l);
 #pragma unroll
-      for (int i = 0; i < W; ++i) o[i] = fmaf(sh[wid + k][W * lane + i], x, o[i]);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(sh[wid + k][2 + e][lane], x, o[e]);
     }
   }
-  if (at / per > pair || parts == 1 || !a.see[(long)b * a.N + r / G]) return;
-  bf16_t* const out = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + W * lane;
+  if (id >= all || parts == 1 || r >= a.N * G || !a.see[(long)b * a.N + r / G]) return;
   const float inv = 1.f / l;
-  if constexpr (W == 2) *(uint32_t*)out = pack2bf(o[0] * inv, o[1] * inv);
-  else out[0] = f2bf(o[0] * inv);
+  *(uint2*)((bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 16 * c + 4 * g) =
+      make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -627,25 +622,25 @@ static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
 template <int D>
 static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
   if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32>(a, rows, stream);
-  else if (rows <= 32) launch_tree_form<D, 1, 2, 1, 64>(a, rows, stream);
-  else if (rows <= 64) launch_tree_form<D, 1, 4, 1, 64>(a, rows, stream);
-  else if (rows <= 128) launch_tree_form<D, 2, 4, 1, 64>(a, rows, stream);
+  else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32>(a, rows, stream);
+  else if (rows <= 64) launch_tree_form<D, 1, 4, 2, 32>(a, rows, stream);
+  else if (rows <= 128) launch_tree_form<D, 2, 4, 2, 32>(a, rows, stream);
   else launch_tree_form<D, 2, 8, 1, 64>(a, rows, stream);
   RT_LAUNCH_CHECK();
   return 0;
 }
 
 template <int D>
-static void launch_join(const TreeArgs& a, long rows, hipStream_t stream) {
-  if (a.S <= 8) hipLaunchKernelGGL((tree_join_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a, 64);
-  else hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a, 64);
+static void launch_join(const TreeArgs& a, long all, hipStream_t stream) {
+  if (a.S <= 8) hipLaunchKernelGGL((tree_join_kernel<D, 1>), dim3((unsigned)((all + 3) / 4)), dim3(256), 0, stream, a, 64);
+  else hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)all), dim3(256), 0, stream, a, 64);
 }
 
 // parts that a row's keys may be cut in: the partials that rt_tree_attention wants. 0: sizes without matrix instructions
 extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax) {
   if ((D != 64 && D != 128) || B == 0) return 0;
   const int stages = (Smax + 63) / 64 + 1, blocks = B * Hkv * ((N * (Hq / Hkv) + 255) / 256);
-  return std::max(1, std::min((2 * num_cus() + blocks - 1) / blocks, (stages + 1) / 2));
+  return std::max(1, std::min((num_cus() + blocks / 2) / blocks, stages));
 }
 
 extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const int* kv_len, const int* kv_start,
@@ -668,7 +663,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
-    const long all = (long)B * Hkv * rows;
+    const long all = (long)B * Hkv * ((rows + 15) / 16) * (D / 16);
     if (D == 128) launch_join<128>(a, all, stream);
     else launch_join<64>(a, all, stream);
     RT_LAUNCH_CHECK();
