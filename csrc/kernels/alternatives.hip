@@ -93,6 +93,9 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
   const long row = blockIdx.x;
   const T* const x = logits + row * ld;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, chunks = (V + E - 1) / E;
+  // the given token's logit, with the row: behind the sums it would be two more trips to memory
+  const int64_t given = tgt ? tgt[row] : -1;
+  const float given_l = get(x + (given >= 0 && given < V ? given : 0));
   u32x4 data[KEEP];
   float top_of[KEEP];
   if constexpr (NC > 0) {
@@ -192,8 +195,7 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
   const float ls = none ? 0.f : __logf(s), mean = none ? 0.f : t / s * LN2;
   auto log_prob = [&](float l) { return none ? -INFINITY : (l - ref) * c2 * LN2 - ls; };
   if (tid == 0) {
-    const int64_t g = tgt ? tgt[row] : -1;
-    logp[row] = g < 0 ? 0.f : g >= V ? NAN : log_prob(get(x + g));
+    logp[row] = given < 0 ? 0.f : given >= V ? NAN : log_prob(given_l);
     ent[row] = ls - mean;
     if (stats) { stats[row * 3] = none ? INFINITY : ref; stats[row * 3 + 1] = ls; stats[row * 3 + 2] = mean; }
   }
@@ -242,7 +244,15 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
     for (int i = tid; i < n; i += THREADS) {
       const uint64_t o = cand[i];
       int before = 0;
-      for (int j = 0; j < n; ++j) before += cand[j] > o;
+      int j = 0;
+      for (; j + 8 <= n; j += 8) {  // eight under way: they come one by one otherwise, 50 of them in a microsecond
+        uint64_t c8[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) c8[q] = cand[j + q];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) before += c8[q] > o;
+      }
+      for (; j < n; ++j) before += cand[j] > o;
       if (before < top) {
         ids[row * top + before] = (int)~(uint32_t)o;
         top_lp[row * top + before] = log_prob(value(o));
@@ -282,26 +292,36 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
                                                                T* __restrict__ d, long ldd, int span) {
   constexpr int E = Chunk<T>::E, MARKS = 4096;
   __shared__ int at[MAX_TOP + 1];
-  __shared__ float up[MAX_TOP + 1];
+  __shared__ float up[MAX_TOP + 1], total_s;
   __shared__ unsigned marks[MARKS / 32];
   const long row = blockIdx.x;
   const T* const x = logits + row * ld;
   T* const dx = d + row * ldd;
-  const int tid = threadIdx.x, chunks = (V + E - 1) / E;
+  const int tid = threadIdx.x, chunks = (V + E - 1) / E, first = blockIdx.y * span, last = min(first + span, chunks), full = V / E;
+  u32x4 w[4];  // the first four chunks, on their way while the row's marks are made
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    w[k] = u32x4{};
+    if (full) __builtin_memcpy(&w[k], x + (long)min(first + tid + k * 256, full - 1) * E, 16);
+  }
   const float m = stats[row * 3], ls = stats[row * 3 + 1], mean = stats[row * 3 + 2];
   if (tid < MARKS / 32) marks[tid] = 0;
   __syncthreads();
-  if (tid <= top) {
-    const int64_t t = tid < top ? ids[row * top + tid] : tgt ? tgt[row] : -1;
-    const bool given = t >= 0 && t < V;
-    at[tid] = given ? (int)t : -1;
-    up[tid] = !given ? 0.f : tid < top ? (g_top ? g_top[row * top + tid] : 0.f) : (g_lp ? g_lp[row] : 0.f);
-    if (given) atomicOr(&marks[(int)t / E % MARKS / 32], 1u << (t / E % 32));
+  if (tid < 64) {
+    float mine = 0.f;
+    if (tid <= top) {
+      const int64_t t = tid < top ? ids[row * top + tid] : tgt ? tgt[row] : -1;
+      const bool given = t >= 0 && t < V;
+      at[tid] = given ? (int)t : -1;
+      mine = !given ? 0.f : tid < top ? (g_top ? g_top[row * top + tid] : 0.f) : (g_lp ? g_lp[row] : 0.f);
+      up[tid] = mine;
+      if (given) atomicOr(&marks[(int)t / E % MARKS / 32], 1u << (t / E % 32));
+    }
+    mine = wave_sum(mine);
+    if (tid == 0) total_s = mine;
   }
   __syncthreads();
-  float total = 0.f;
-  for (int k = 0; k <= top; ++k) total += up[k];
-  const float ge = g_ent ? g_ent[row] : 0.f, c2 = c * LOG2E, ls2 = ls * LOG2E;
+  const float total = total_s, ge = g_ent ? g_ent[row] : 0.f, c2 = c * LOG2E, ls2 = ls * LOG2E;
   const bool none = m == INFINITY && ls == 0.f;
   // -c p (total + g_H (z - mean)) with z in steps of log 2
   const float k1 = none ? 0.f : -c * (total - ge * mean), k2 = none ? 0.f : -c * ge * LN2;
@@ -323,8 +343,8 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
     }
     if ((ch + 1) * E <= V) {
       if constexpr (E == 8) {
-        const uint4 w = pack8(f);
-        __builtin_memcpy(dx + (long)ch * E, &w, 16);
+        const uint4 out = pack8(f);
+        __builtin_memcpy(dx + (long)ch * E, &out, 16);
       } else {
         __builtin_memcpy(dx + (long)ch * E, f, 16);
       }
@@ -334,14 +354,22 @@ __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restri
         if (ch * E + i < V) put(dx + (long)ch * E + i, f[i]);
     }
   };
-  const int first = blockIdx.y * span, last = min(first + span, chunks);
+  const int whole = min(last, full);
   int ch = first + tid;
-  for (; ch + 3 * 256 < min(last, V / E); ch += 4 * 256) {
-    u32x4 w[4];
+  for (; ch + 3 * 256 < whole; ch += 4 * 256) {
+    if (ch != first + tid) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) __builtin_memcpy(&w[k], x + (long)(ch + k * 256) * E, 16);
+      for (int k = 0; k < 4; ++k) __builtin_memcpy(&w[k], x + (long)(ch + k * 256) * E, 16);
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) one(ch + k * 256, w[k]);
+  }
+  if (ch == first + tid) {  // less than four of them
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (ch + k * 256 < whole) one(ch + k * 256, w[k]);
+    if (full < last && full >= first && (full - first) % 256 == tid) one(full, load_tail(x, full, V));
+    return;
   }
   for (; ch < last; ch += 256) one(ch, load_chunk(x, ch, V));
 }

@@ -5,6 +5,7 @@
 #include "rt_paged.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace rt {
@@ -54,6 +55,7 @@ struct TreeArgs {
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
   int sorted;
+  float part_cost, join_cost;           // in stages
   float* part; int S;                   // partials of at most S shares of a row's keys (part_of)
 };
 
@@ -130,6 +132,17 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
 // lanes, and p goes from the scores' registers to the product's as it is (rounded to the cache's type: half a step of bf16 for each term,
 // the sums in fp32). WR waves share the rows, RT tiles of 16 each, WK the keys of a stage.
 // Shares of a long row's keys (cut(): by the lengths, which only the device knows) leave fp32 partials that a second launch joins.
+// How many of a row's stages one part takes. Parts of `per` stages cost, in stages, per + part_cost * parts + join_cost: each part writes and reads
+// partials of all rows of its key head, whatever its length. Measured: 16 nodes of one row over 4096 keys in 8 key heads (65 stages) 17.1 /
+// 14.9 / 13.9 / 16.0 us in 8 / 16 / 22 / 33 parts, 48 rows of 150 to 1200 keys 31 / 44 / 50 in 1 / 2 / 3.
+__host__ __device__ inline int stages_per_part(int stages, int most, float part_cost, float join_cost) {
+  if (most <= 1 || stages <= 1) return stages > 1 ? stages : 1;
+  int per = (int)(sqrtf(stages * part_cost) + 0.5f), least = (stages + most - 1) / most;
+  per = per < least ? least : per;
+  const int parts = (stages + per - 1) / per;
+  return parts > 1 && per + part_cost * parts + join_cost < stages ? per : stages;
+}
+
 struct Cut { int lo, len, tiles, parts, per; };  // tiles: stages of the context and the nodes' one
 __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int SK) {
   Cut c;
@@ -138,7 +151,7 @@ __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int SK) {
   if (a.window) c.lo = max(c.lo, c.len - a.window + 1);
   c.lo = min(c.lo, c.len);
   c.tiles = (c.len - c.lo + SK - 1) / SK + 1;
-  c.per = (c.tiles + a.S - 1) / a.S;
+  c.per = stages_per_part(c.tiles, a.S, a.part_cost, a.join_cost);
   c.parts = (c.tiles + c.per - 1) / c.per;
   return c;
 }
@@ -316,7 +329,6 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
               if (key >= ct.len || key < from[u]) st[k][u][e] = -INFINITY;
             }
       }
-      float alpha[RT];
       bool grown = false;
       float mn[RT];
 #pragma unroll
@@ -327,7 +339,9 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx = larger(mx, st[k][u][e]);
         mn[u] = larger(m[u], over_groups(mx, [](float p, float q) { return larger(p, q); }));
-        grown = grown || !((mn[u] - m[u]) * a.scale <= 8.f || mn[u] == m[u]);
+        // each row by its own growth, so that what a row gives does not depend on the rows beside it
+        if ((mn[u] - m[u]) * a.scale <= 8.f || mn[u] == m[u]) mn[u] = m[u];
+        else grown = true;
       }
       // the maximum that p is taken from follows the rows' own only by steps: up to 2^8 instead of 1 costs nothing in fp32, and o is seldom
       // multiplied
@@ -335,11 +349,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
 #pragma unroll
         for (int u = 0; u < RT; ++u) {
           const float mz = (mn[u] == -INFINITY ? 0.f : mn[u]) * a.scale;  // a row may see nothing of its first stages
-          alpha[u] = paged::fexp2(m[u] * a.scale - mz);
+          const float x = mn[u] == m[u] ? 1.f : paged::fexp2(m[u] * a.scale - mz);
           m[u] = mn[u];
-          l[u] *= alpha[u];
+          l[u] *= x;
 #pragma unroll
-          for (int c = 0; c < DT; ++c) o[u][c] *= alpha[u];
+          for (int c = 0; c < DT; ++c) o[u][c] *= x;
         }
       }
 #pragma unroll
@@ -636,11 +650,23 @@ static void launch_join(const TreeArgs& a, long all, hipStream_t stream) {
   else hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)all), dim3(256), 0, stream, a, 64);
 }
 
-// parts that a row's keys may be cut in: the partials that rt_tree_attention wants. 0: sizes without matrix instructions
+// a stage's time in us (one workgroup on a CU), a part's of all key heads and a join's in such times
+static void tree_costs(int B, int N, int Hq, int Hkv, int D, float& part, float& join) {
+  const int rows = N * (Hq / Hkv);
+  const float stage = (rows <= 64 ? 0.9f : rows <= 128 ? 1.2f : 2.4f) * (D == 64 ? 0.7f : 1.f);
+  part = (float)B * Hkv * ((rows + 15) / 16 * 16) * (D + 2) * 8 / 4.5e6f / stage;
+  join = 3.f / stage;
+}
+
+// Parts that a row's keys may be cut in at most: the partials that rt_tree_attention wants (0: sizes without matrix instructions). As many as
+// fill the CUs once; 1, and no second launch, where a full cache would not be cut.
 extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax) {
   if ((D != 64 && D != 128) || B == 0) return 0;
   const int stages = (Smax + 63) / 64 + 1, blocks = B * Hkv * ((N * (Hq / Hkv) + 255) / 256);
-  return std::max(1, std::min((num_cus() + blocks / 2) / blocks, stages));
+  const int most = std::max(1, std::min((num_cus() + blocks / 2) / blocks, stages));
+  float part, join;
+  tree_costs(B, N, Hq, Hkv, D, part, join);
+  return stages_per_part(stages, most, part, join) < stages ? most : 1;
 }
 
 extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const int* kv_len, const int* kv_start,
@@ -648,7 +674,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
                                  int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, part, S};
+  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, 0.f, 0.f, part, S};
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
     if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
@@ -658,6 +684,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   }
   if (f32 || (D != 64 && D != 128) || (S > 1 && !part)) return -1;
   a.scale = scale * 1.4426950408889634f;
+  tree_costs(B, N, Hq, Hkv, D, a.part_cost, a.join_cost);
   const int rows = N * (Hq / Hkv);
   a.sorted = B > 1 && B <= 64 && (long)B * Hkv * S * ((rows + 255) / 256) > num_cus();
   const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
