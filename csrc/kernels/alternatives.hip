@@ -119,6 +119,7 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
     if constexpr (NC > 0) {
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
+        if (k * THREADS >= chunks) break;
         asm volatile("" : "+v"(data[k]));  // opened anew in each pass: kept open it takes twice the registers
         f(k, k * THREADS + tid, data[k]);
       }
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
     unsigned hits = 0;
     const int q = tch >= tid ? (tch - tid) / THREADS : -1;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) hits |= (top_of[k] > tv || (top_of[k] == tv && k <= q) ? 1u : 0u) << k;
+    for (int k = 0; k < NC; ++k) if (k * THREADS < chunks) hits |= (top_of[k] > tv || (top_of[k] == tv && k <= q) ? 1u : 0u) << k;
     for (; hits; hits &= hits - 1) {
       const int ch = __builtin_ctz(hits) * THREADS + tid;
       if (ch < chunks) look(ch, load_chunk(x, ch, V));
@@ -283,95 +284,83 @@ __global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restri
 }
 
 // dl = c (up - p (sum up) - g_H p (z - mean)), up: the given token's and the alternatives' gradients at their places. A row is read and
-// written once; the few chunks with such places are known by a bit of their index (others may share it: they look and find nothing).
+// written once; the places with gradients of their own, 33 at most, are written again behind the chunks that hold them.
 template <typename T>
 __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
                                                                int V, int top, const int64_t* __restrict__ ids,
                                                                const float* __restrict__ stats, const float* __restrict__ g_lp,
                                                                const float* __restrict__ g_ent, const float* __restrict__ g_top,
-                                                               T* __restrict__ d, long ldd, int span) {
-  constexpr int E = Chunk<T>::E, MARKS = 4096;
-  __shared__ int at[MAX_TOP + 1];
-  __shared__ float up[MAX_TOP + 1], total_s;
-  __shared__ unsigned marks[MARKS / 32];
+                                                               T* d, long ldd, int span) {
+  constexpr int E = Chunk<T>::E;
+  __shared__ float total_s;
   const long row = blockIdx.x;
   const T* const x = logits + row * ld;
   T* const dx = d + row * ldd;
-  const int tid = threadIdx.x, chunks = (V + E - 1) / E, first = blockIdx.y * span, last = min(first + span, chunks), full = V / E;
-  u32x4 w[4];  // the first four chunks, on their way while the row's marks are made
+  const int tid = threadIdx.x, chunks = (V + E - 1) / E, full = V / E;
+  const int first = blockIdx.y * span, last = min(first + span, chunks), whole = min(last, full);
+  u32x4 w[4];  // the first four chunks, on their way while the row's gradients are added
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     w[k] = u32x4{};
     if (full) __builtin_memcpy(&w[k], x + (long)min(first + tid + k * 256, full - 1) * E, 16);
   }
   const float m = stats[row * 3], ls = stats[row * 3 + 1], mean = stats[row * 3 + 2];
-  if (tid < MARKS / 32) marks[tid] = 0;
-  __syncthreads();
+  int place = -1;
+  float up = 0.f, at_place = 0.f;
   if (tid < 64) {
-    float mine = 0.f;
     if (tid <= top) {
       const int64_t t = tid < top ? ids[row * top + tid] : tgt ? tgt[row] : -1;
-      const bool given = t >= 0 && t < V;
-      at[tid] = given ? (int)t : -1;
-      mine = !given ? 0.f : tid < top ? (g_top ? g_top[row * top + tid] : 0.f) : (g_lp ? g_lp[row] : 0.f);
-      up[tid] = mine;
-      if (given) atomicOr(&marks[(int)t / E % MARKS / 32], 1u << (t / E % 32));
+      place = t >= 0 && t < V ? (int)t : -1;
+      up = place < 0 ? 0.f : tid < top ? (g_top ? g_top[row * top + tid] : 0.f) : (g_lp ? g_lp[row] : 0.f);
+      at_place = get(x + max(place, 0));
     }
-    mine = wave_sum(mine);
-    if (tid == 0) total_s = mine;
+    const float total = wave_sum(up);
+    if (tid == 0) total_s = total;
+    // a given token that is among the alternatives adds to its place there
+    const int given = __builtin_amdgcn_readlane(place, top);
+    const float given_up = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(up), top));
+    const bool among = tid < top && place == given && given >= 0;
+    if (among) up += given_up;
+    if (__any(among) && tid == top) place = -1;
   }
   __syncthreads();
   const float total = total_s, ge = g_ent ? g_ent[row] : 0.f, c2 = c * LOG2E, ls2 = ls * LOG2E;
   const bool none = m == INFINITY && ls == 0.f;
   // -c p (total + g_H (z - mean)) with z in steps of log 2
   const float k1 = none ? 0.f : -c * (total - ge * mean), k2 = none ? 0.f : -c * ge * LN2;
-  auto one = [&](int ch, const u32x4& w) {
+  auto slope = [&](float l) {
+    const float z = (l - m) * c2;
+    return __builtin_amdgcn_exp2f(z - ls2) * fmaf(k2, fmaxf(z, -1e30f), k1);
+  };
+  auto one = [&](int ch, const u32x4& in) {
     float f[E];
-    Chunk<T>::open(w, f);
+    Chunk<T>::open(in, f);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float z = (f[i] - m) * c2, p = __builtin_amdgcn_exp2f(z - ls2);
-      f[i] = p * fmaf(k2, fmaxf(z, -1e30f), k1);
-    }
-    if (marks[ch % MARKS / 32] >> (ch % 32) & 1) {
-      for (int k = 0; k <= top; ++k) {
-        const int i0 = at[k] - ch * E;
-        if (at[k] >= 0 && i0 >= 0 && i0 < E)
-#pragma unroll
-          for (int i = 0; i < E; ++i) f[i] += i == i0 && !none ? c * up[k] : 0.f;
-      }
-    }
-    if ((ch + 1) * E <= V) {
-      if constexpr (E == 8) {
-        const uint4 out = pack8(f);
-        __builtin_memcpy(dx + (long)ch * E, &out, 16);
-      } else {
-        __builtin_memcpy(dx + (long)ch * E, f, 16);
-      }
+    for (int i = 0; i < E; ++i) f[i] = slope(f[i]);
+    if constexpr (E == 8) {
+      const uint4 out = pack8(f);
+      __builtin_memcpy(dx + (long)ch * E, &out, 16);
     } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (ch * E + i < V) put(dx + (long)ch * E + i, f[i]);
+      __builtin_memcpy(dx + (long)ch * E, f, 16);
     }
   };
-  const int whole = min(last, full);
-  int ch = first + tid;
-  for (; ch + 3 * 256 < whole; ch += 4 * 256) {
-    if (ch != first + tid) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) __builtin_memcpy(&w[k], x + (long)(ch + k * 256) * E, 16);
-    }
+  for (int k = 0; k < 4; ++k)
+    if (first + tid + k * 256 < whole) one(first + tid + k * 256, w[k]);
+  int ch = first + tid + 4 * 256;
+  for (; ch + 3 * 256 < whole; ch += 4 * 256) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) __builtin_memcpy(&w[k], x + (long)(ch + k * 256) * E, 16);
 #pragma unroll
     for (int k = 0; k < 4; ++k) one(ch + k * 256, w[k]);
   }
-  if (ch == first + tid) {  // less than four of them
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (ch + k * 256 < whole) one(ch + k * 256, w[k]);
-    if (full < last && full >= first && (full - first) % 256 == tid) one(full, load_tail(x, full, V));
-    return;
+  for (; ch < whole; ch += 256) {
+    __builtin_memcpy(&w[0], x + (long)ch * E, 16);
+    one(ch, w[0]);
   }
-  for (; ch < last; ch += 256) one(ch, load_chunk(x, ch, V));
+  if (last > full && tid < V - full * E) put(dx + full * E + tid, slope(get(x + full * E + tid)));  // less than a chunk
+  __syncthreads();
+  if (place >= first * E && place < last * E) put(dx + place, none ? 0.f : fmaf(c, up, slope(at_place)));
 }
 
 }  // namespace alt
