@@ -1,6 +1,7 @@
 // Python bindings of the kernels that check drafted tokens (csrc/kernels/drafts.hip, alternatives.hip): checked wrappers on the current
 // stream of the operands' device. Parents, lengths and targets are bounded inside the kernels.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -89,11 +90,14 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   const double scale = scale_.has_value() ? *scale_ : 1 / std::sqrt((double)D);
   TORCH_CHECK_VALUE(window >= 0 && scale > 0 && std::isfinite(scale), "tree_attention: window ", window, ", scale ", scale);
   TORCH_CHECK_VALUE(D <= 512 && Smax * D < (1L << 30) && window < (1L << 30) && Hq < 65536 && B < 65536, "tree_attention: sizes");
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(qkv.requires_grad() || kc.requires_grad() || vc.requires_grad()),
+                    "tree_attention has no gradient");
   const c10::DeviceGuard guard(qkv.device());
   const Tensor out = has(out_) ? *out_ : at::empty({B * N, Hq * D}, qkv.options());
   on(out, qkv, "tree_attention out");
   TORCH_CHECK_VALUE(out.scalar_type() == qkv.scalar_type() && out.dim() == 2 && out.size(0) == B * N && out.size(1) == Hq * D &&
                         (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
+  at::assert_no_overlap(out, qkv);
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax) : 0;
   // matrix instructions want rows at 16 bytes (the output at 8): others are copied
@@ -169,8 +173,8 @@ struct AlternativesFn : torch::autograd::Function<AlternativesFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor logits = saved[0], targets = saved[1], ids = saved[2], stats = saved[3];
     const int64_t T = logits.size(0), V = logits.size(1);
+    TORCH_CHECK(!at::GradMode::is_enabled(), "token_alternatives has no second derivative");
     for (int i = 0; i < 3; ++i) {
-      TORCH_CHECK(!grads[i].defined() || !grads[i].requires_grad() || !at::GradMode::is_enabled(), "token_alternatives has no second derivative");
       if (grads[i].defined()) grads[i] = grads[i].to(at::kFloat).contiguous();
     }
     auto g = [&](int i) { return grads[i].defined() ? grads[i].data_ptr<float>() : nullptr; };

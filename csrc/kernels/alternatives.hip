@@ -80,7 +80,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // where 20 are wanted); each counts how many of the others are before it. Where they are more than CAP (rows made for it) the
 // best are taken one by one.
 template <typename T, int THREADS, int NC>
-__global__ __launch_bounds__(THREADS) void alternatives_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
+__global__ __launch_bounds__(THREADS, NC ? 1 : 8) void alternatives_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
                                                                int V, int top, float* __restrict__ logp, float* __restrict__ ent,
                                                                float* __restrict__ top_lp, int64_t* __restrict__ ids,
                                                                float* __restrict__ stats) {

@@ -474,7 +474,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 4 * g;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
-          *(uint2*)(p + 16 * c) = make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv));
+          *(uint2*)(p + 16 * c) = sees[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
+                                          : make_uint2(0, 0);
       }
     }
   }
@@ -549,10 +550,11 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
       for (int e = 0; e < 4; ++e) o[e] = fmaf(sh[wid + k][2 + e][lane], x, o[e]);
     }
   }
-  if (id >= all || parts == 1 || r >= a.N * G || !a.see[(long)b * a.N + r / G]) return;
+  if (id >= all || parts == 1 || r >= a.N * G) return;
+  const bool node = a.see[(long)b * a.N + r / G] != 0;  // others have no parts
   const float inv = 1.f / l;
   *(uint2*)((bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 16 * c + 4 * g) =
-      make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv));
+      node ? make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)) : make_uint2(0, 0);
 }
 
 // ---------------------------------------------------------------------------------------------

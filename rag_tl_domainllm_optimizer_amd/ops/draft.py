@@ -73,8 +73,10 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
         raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}: an fp8 cache is read by decode_step_attention only")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
-    if window < 0 or not scale > 0:
+    if window < 0 or not 0 < scale < math.inf:
         raise ValueError(f"window {window}, scale {scale}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (qkv, k_cache, v_cache)):
+        raise ValueError("tree_attention has no gradient")
     kv_len = _ints(kv_len, "kv_len", (B,), qkv)
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
     o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale)

@@ -128,6 +128,9 @@ def test_alternatives_of_masked_rows_have_finite_gradients():
     lambda: _attend(qkv=torch.zeros(5, 32)),
     lambda: _attend(qkv=torch.zeros(6, 31)),
     lambda: _attend(window=-1),
+    lambda: _attend(scale=0.0),
+    lambda: _attend(scale=math.nan),
+    lambda: _attend(qkv=torch.zeros(6, 32, requires_grad=True)),
     lambda: _attend(kc=torch.zeros(2, 2, 9, 4, dtype=torch.uint8)),
     lambda: _attend(kv_len=torch.zeros(2, dtype=torch.int64)),
     lambda: _attend(kv_start=torch.zeros(3, dtype=torch.int32)),
@@ -151,11 +154,11 @@ def test_refused(bad):
         bad()
 
 
-def _attend(qkv=None, kc=None, kv_len=None, kv_start=None, Hq=4, window=0):
+def _attend(qkv=None, kc=None, kv_len=None, kv_start=None, Hq=4, window=0, scale=None):
     z = torch.zeros
     kc = z(2, 2, 9, 4) if kc is None else kc
     return ops.tree_attention(z(6, 32) if qkv is None else qkv, kc, kc, z(2, dtype=torch.int32) if kv_len is None else kv_len,
-                              _tree([[-1, 0, 0]] * 2), Hq, kv_start, window)
+                              _tree([[-1, 0, 0]] * 2), Hq, kv_start, window, scale)
 
 
 def _accept(tokens=None, choice=None, drafts=None, kv_len=None):

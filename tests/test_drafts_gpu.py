@@ -149,6 +149,35 @@ def test_attention_lengths_past_the_cache_and_below_zero():
     assert torch.equal(c, ops.tree_attention(qkv, kc, vc, _i32([0, 0]), tree, 4))
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,slots", [(8, 2, 128, 2000), (8, 2, 128, 60), (3, 1, 32, 60)])
+def test_attention_of_masks_with_holes(Hq, Hkv, D, slots):
+    """a plan of the caller's own: nodes that see nothing between others, and nodes that see others than ancestors"""
+    N = 12
+    see = [1, 0, 0b101, 0, 0, 0b100100, 1 << 6, 0, 0b111111000001 & 0b000100000001, 0, 0b10000000101, 0]
+    see = [s if s == 0 else s | 1 << i for i, s in enumerate(see)]
+    qkv, kc, vc = _rand(N, (Hq + 2 * Hkv) * D, seed=1), _rand(1, Hkv, slots, D, seed=2), _rand(1, Hkv, slots, D, seed=3)
+    tree = ops.DraftTree(_i32([[-1] * N]), torch.tensor([see], device=DEV), _i32([[0] * N]))
+    o = ops.tree_attention(qkv, kc, vc, _i32([slots]), tree, Hq)
+    want = ops.tree_attention(qkv.cpu().double(), kc.cpu().double(), vc.cpu().double(), torch.tensor([slots], dtype=torch.int32),
+                              ops.DraftTree(*(t.cpu() for t in (tree.parent, tree.see, tree.pos))), Hq)
+    assert (o[[i for i, s in enumerate(see) if not s]] == 0).all()
+    # two roundings of half a step, of p in a mean of |v| below 1 and of the output below 2 here, and scores as in _attention
+    assert ((o.cpu().double() - want).abs() <= 2 ** -8 * (1 + want.abs()) + 2 * 2 ** -24 * (16 * D + slots)).all()
+
+
+def test_attention_gives_a_row_the_same_beside_others():
+    """a row's bits do not depend on the other rows of the batch, nor a node's on the nodes that it does not see"""
+    B, N, Hq, Hkv, D = 3, 10, 8, 2, 128
+    qkv, kc, vc = _rand(B * N, (Hq + 2 * Hkv) * D), _rand(B, Hkv, 500, D, seed=1), _rand(B, Hkv, 500, D, seed=2)
+    lens, parents = [490, 3, 200], plain.trees(B, N, 0)
+    a = ops.tree_attention(qkv, kc, vc, _i32(lens), ops.draft_tree(_i32(parents)), Hq)
+    others = qkv.clone()
+    others[N:] *= 30  # the other rows' queries and keys
+    others[N - 1] *= 30  # the last node of row 0: nobody's ancestor
+    b = ops.tree_attention(others, kc, vc, _i32([490, 400, 1]), ops.draft_tree(_i32(parents)), Hq)
+    assert torch.equal(a[:N - 1], b[:N - 1])
+
+
 def test_attention_nothing_to_do():
     tree = ops.draft_tree(torch.zeros(0, 3, dtype=torch.int32, device=DEV))
     o = ops.tree_attention(torch.zeros(0, 512, dtype=BF16, device=DEV), *(torch.zeros(0, 2, 9, 64, dtype=BF16, device=DEV) for _ in "kv"), _i32([]), tree, 4)
@@ -415,6 +444,34 @@ def test_steps_on_two_streams_at_once():
                 assert torch.equal(a, b)
 
 
+def test_a_captured_gradient_replays():
+    x, t = _rand(9, 1003, dtype=F32, seed=1), torch.arange(-1, 8, device=DEV)
+    g = [_rand(9, dtype=F32, seed=2), _rand(9, dtype=F32, seed=3), _rand(9, 5, dtype=F32, seed=4)]
+
+    def step(x):
+        y = x.detach().requires_grad_(True)
+        lp, ent, top, ids = ops.token_alternatives(y, t, 5, 1.1)
+        return lp.detach(), ent.detach(), top.detach(), ids, torch.autograd.grad([lp, ent, top], y, g)[0]
+
+    held, runner, work = {}, GraphRunner(), x.clone()
+    runner.capture(lambda: held.update(out=step(work)), "step")
+    for seed in (1, 5, 6):
+        new = _rand(9, 1003, dtype=F32, seed=seed)
+        work.copy_(new)
+        runner.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in held["out"]]
+        for a, b in zip(got, step(new)):
+            assert torch.equal(a, b)
+
+
+def test_no_second_derivative():
+    x = _rand(2, 50, dtype=F32).requires_grad_(True)
+    lp = ops.token_alternatives(x, torch.tensor([1, 2], device=DEV), 2)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(lp.sum(), x, create_graph=True)
+
+
 def test_runs_repeat_bit_by_bit():
     qkv, kc, vc = _rand(8 * 20, 12 * 128, seed=1), _rand(8, 2, 3000, 128, seed=2), _rand(8, 2, 3000, 128, seed=3)
     tree, lens = ops.draft_tree(_i32(plain.trees(8, 20, 0))), _i32([3000, 1, 700, 0, 64, 2999, 1500, 33])
@@ -438,6 +495,13 @@ def test_runs_repeat_bit_by_bit():
                                out=torch.empty(2, 255, dtype=BF16, device=DEV)),
     lambda: ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.long, device=DEV) for _ in "tc"), [_rand(2, 512)],
                             _rand(1, 1, 2, 9, 64), _rand(1, 1, 2, 64, 9).transpose(3, 4), _i32([3])),
+    lambda: ops.tree_attention(_rand(2, 512).requires_grad_(True), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4),
+    lambda: ops.tree_attention(_rand(2, 512), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, scale=-1.0),
+    lambda: ops.tree_attention(_rand(2, 512), *(torch.zeros(1, 2, 9, 64, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4),
+    lambda: ops.draft_tree(torch.zeros(2, 65, dtype=torch.int32, device=DEV)),
+    lambda: ops.token_alternatives(_rand(2, 50), None, 33),
+    lambda: ops.token_alternatives(_rand(2, 50), None, 2, math.inf),
+    lambda: ops.token_alternatives(_rand(2, 50), torch.zeros(3, dtype=torch.long, device=DEV), 2),
     lambda: ops.token_alternatives(_rand(2, 50).half(), None, 2),
     lambda: ops.token_alternatives(_rand(2, 50), torch.zeros(2, dtype=torch.long), 2),
 ])
