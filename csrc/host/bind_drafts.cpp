@@ -12,7 +12,7 @@
 
 extern "C" {
 int rt_draft_tree(const int*, const int*, const int*, int, int, int64_t*, int*, hipStream_t);
-int rt_tree_parts(int, int, int, int, int, int);
+int rt_tree_parts(int, int, int, int, int, int, int);
 int rt_tree_attention(int, const void*, long, const void*, const void*, const int*, const int*, const int64_t*, void*, long, float*, int, int,
                       int, int, int, int, int, int, float, hipStream_t);
 int rt_tree_accept(const int*, const int64_t*, const int64_t*, const int64_t*, const int*, int*, int*, int64_t*, const void* const*, long, void*,
@@ -99,7 +99,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
                         (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
   at::assert_no_overlap(out, qkv);
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
-                        ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax) : 0;
+                        ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window) : 0;
   // matrix instructions want rows at 16 bytes (the output at 8): others are copied
   Tensor x = qkv, o = out;
   if (S && !(al(x, 16) && x.stride(0) % 8 == 0 && x.stride(0) < (1L << 24))) x = qkv.narrow(1, 0, (Hq + 2 * Hkv) * D).clone(at::MemoryFormat::Contiguous);

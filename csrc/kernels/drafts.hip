@@ -54,7 +54,7 @@ struct TreeArgs {
   void* o; long ldo;
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
-  int sorted;
+  int sorted, blocks;                   // long rows first; workgroups for a key head's rows
   float part_cost, join_cost;           // in stages
   float* part; int S;                   // partials of at most S shares of a row's keys (part_of)
 };
@@ -190,7 +190,10 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
   __shared__ unsigned bad[2];  // nodes whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
-  const int s = blockIdx.x % a.S, pair = blockIdx.x / a.S % (a.B * a.Hkv), rb = blockIdx.x / a.S / (a.B * a.Hkv);
+  // blocks go to the eight XCDs in turn: those that read the same keys for other rows come eight later, to the same L2
+  const int lin = a.blocks == 1 ? blockIdx.x : blockIdx.x / (8 * a.blocks) * 8 + blockIdx.x % 8, rb = a.blocks == 1 ? 0 : blockIdx.x / 8 % a.blocks;
+  const int s = lin % a.S, pair = lin / a.S;
+  if (pair >= a.B * a.Hkv) return;
   const int b = a.sorted ? longest(a, pair / a.Hkv, lane) : pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
   const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
   const uint64_t live = __ballot(see != 0);
@@ -630,17 +633,25 @@ extern "C" int rt_draft_tree(const int* parent, const int* nodes, const int* pos
   return 0;
 }
 
+constexpr int WIDE_ROWS = 192;  // rows of a key head that go to workgroups of 64
+
 template <int D, int RT, int WR, int WK, int KT>
 static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
-  const int blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
-  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), dim3((unsigned)(a.S * a.B * a.Hkv * blocks)), dim3(64 * WR * WK), 0, stream, a);
+  TreeArgs t = a;
+  t.blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
+  const int all = a.S * a.B * a.Hkv;
+  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), dim3((unsigned)(t.blocks == 1 ? all : (all + 7) / 8 * 8 * t.blocks)), dim3(64 * WR * WK),
+                     0, stream, t);
 }
 template <int D>
 static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
+  // waves by rows of 16, and two shares of each stage's keys: half the chain of a stage, and the shares are joined in LDS at the end (16 ungrouped
+  // rows of 32 nodes 52 -> 47 us, 48 rows of 64 34 -> 31 against one share). Up to 192 rows go to workgroups of 64, two of them on a
+  // CU, that read the same keys from L2 (32 rows of 128 over 500 to 2900 keys 56 us, in one workgroup of 8 waves with two tiles each 64); beyond, and
+  // with few idle waves, two tiles a wave halve the reads of LDS (40 rows of 240 41 us against 46).
   if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32>(a, rows, stream);
   else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32>(a, rows, stream);
-  else if (rows <= 64) launch_tree_form<D, 1, 4, 2, 32>(a, rows, stream);
-  else if (rows <= 128) launch_tree_form<D, 2, 4, 2, 32>(a, rows, stream);
+  else if (rows <= WIDE_ROWS) launch_tree_form<D, 1, 4, 2, 32>(a, rows, stream);
   else launch_tree_form<D, 2, 8, 1, 64>(a, rows, stream);
   RT_LAUNCH_CHECK();
   return 0;
@@ -652,23 +663,26 @@ static void launch_join(const TreeArgs& a, long all, hipStream_t stream) {
   else hipLaunchKernelGGL((tree_join_kernel<D, 4>), dim3((unsigned)all), dim3(256), 0, stream, a, 64);
 }
 
-// a stage's time in us (one workgroup on a CU), a part's of all key heads and a join's in such times
+// a part's time of all key heads and a join's, in stages (0.9 us of a workgroup that is alone on its CU, 2.4 with 256 rows)
 static void tree_costs(int B, int N, int Hq, int Hkv, int D, float& part, float& join) {
   const int rows = N * (Hq / Hkv);
-  const float stage = (rows <= 64 ? 0.9f : rows <= 128 ? 1.2f : 2.4f) * (D == 64 ? 0.7f : 1.f);
+  const float stage = (rows <= WIDE_ROWS ? 0.9f : 2.4f) * (D == 64 ? 0.7f : 1.f);
   part = (float)B * Hkv * ((rows + 15) / 16 * 16) * (D + 2) * 8 / 4.5e6f / stage;
   join = 3.f / stage;
 }
 
-// Parts that a row's keys may be cut in at most: the partials that rt_tree_attention wants (0: sizes without matrix instructions). As many as
-// fill the CUs once; 1, and no second launch, where a full cache would not be cut.
-extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax) {
+// Parts that a row's keys may be cut in at most: the partials that rt_tree_attention wants (0: sizes without matrix instructions). No more than
+// fill the CUs once; 1, and no second launch, where a full cache would not gain a quarter by them (the launch costs 3 us also where no
+// row turns out long enough).
+extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax, int window) {
   if ((D != 64 && D != 128) || B == 0) return 0;
-  const int stages = (Smax + 63) / 64 + 1, blocks = B * Hkv * ((N * (Hq / Hkv) + 255) / 256);
+  const int rows = N * (Hq / Hkv), blocks = B * Hkv * (rows <= WIDE_ROWS ? (rows + 63) / 64 : (rows + 255) / 256);
+  const int stages = ((window ? std::min(Smax, window) : Smax) + 63) / 64 + 1;
   const int most = std::max(1, std::min((num_cus() + blocks / 2) / blocks, stages));
   float part, join;
   tree_costs(B, N, Hq, Hkv, D, part, join);
-  return stages_per_part(stages, most, part, join) < stages ? most : 1;
+  const int per = stages_per_part(stages, most, part, join), parts = (stages + per - 1) / per;
+  return per + part * parts + join < 0.75f * stages ? parts : 1;
 }
 
 extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const int* kv_len, const int* kv_start,
@@ -676,7 +690,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
                                  int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, 0.f, 0.f, part, S};
+  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, 1, 0.f, 0.f, part, S};
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
     if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
@@ -688,7 +702,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   a.scale = scale * 1.4426950408889634f;
   tree_costs(B, N, Hq, Hkv, D, a.part_cost, a.join_cost);
   const int rows = N * (Hq / Hkv);
-  a.sorted = B > 1 && B <= 64 && (long)B * Hkv * S * ((rows + 255) / 256) > num_cus();
+  a.sorted = B > 1 && B <= 64 && (long)B * Hkv * S > num_cus();
   const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
