@@ -143,14 +143,23 @@ __host__ __device__ inline int stages_per_part(int stages, int most, float part_
   return parts > 1 && per + part_cost * parts + join_cost < stages ? per : stages;
 }
 
-struct Cut { int lo, len, tiles, parts, per; };  // tiles: stages of the context and the nodes' one
-__device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int SK) {
+// nodes of a row (those that see nothing lie behind them, or between them in plans of a caller's own); every lane of a wave has to be there
+__device__ __forceinline__ int count_nodes(uint64_t see) {
+  const uint64_t live = __ballot(see != 0);
+  return live ? 64 - __builtin_clzll(live) : 0;
+}
+
+// full: stages that the context fills; rest: its last keys, which go into the nodes' stage where both fit there
+struct Cut { int lo, len, full, rest, tiles, parts, per; };
+__device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int n, int SK) {
   Cut c;
   c.len = min(max(a.kv_len[b], 0), a.Smax);
   c.lo = a.kv_start ? max(a.kv_start[b], 0) : 0;
   if (a.window) c.lo = max(c.lo, c.len - a.window + 1);
   c.lo = min(c.lo, c.len);
-  c.tiles = (c.len - c.lo + SK - 1) / SK + 1;
+  c.full = (c.len - c.lo) / SK;
+  c.rest = (c.len - c.lo) % SK;
+  c.tiles = c.full + (c.rest + n > SK ? 2 : 1);
   c.per = stages_per_part(c.tiles, a.S, a.part_cost, a.join_cost);
   c.parts = (c.tiles + c.per - 1) / c.per;
   return c;
@@ -188,7 +197,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
   static_assert(KB / 1024 % NW == 0 && SK >= NODES);
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
-  __shared__ unsigned bad[2];  // nodes whose values are not all numbers
+  __shared__ unsigned bad[2];  // keys of the nodes' stage whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   // blocks go to the eight XCDs in turn: those that read the same keys for other rows come eight later, to the same L2
   const int lin = a.blocks == 1 ? blockIdx.x : blockIdx.x / (8 * a.blocks) * 8 + blockIdx.x % 8, rb = a.blocks == 1 ? 0 : blockIdx.x / 8 % a.blocks;
@@ -196,9 +205,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   if (pair >= a.B * a.Hkv) return;
   const int b = a.sorted ? longest(a, pair / a.Hkv, lane) : pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
   const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
-  const uint64_t live = __ballot(see != 0);
-  const int n = live ? 64 - __builtin_clzll(live) : 0, M = n * G;
-  const Cut ct = cut(a, b, SK);
+  const int n = count_nodes(see), M = n * G;
+  const Cut ct = cut(a, b, n, SK);
   if (s >= ct.parts) return;
   const int t0 = s * ct.per, t1 = min(t0 + ct.per, ct.tiles);
   const int row0 = rb * ROWS + wr * 16 * RT;  // of this wave
@@ -209,6 +217,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     bf16x8 qf[RT][DS];
     uint64_t sees[RT];
     int from[RT];  // first key of the context that the row sees
+    bool node_of[RT];
+    const int joint = ct.tiles == ct.full + 1 ? ct.rest : 0;
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
       const int r = min(row0 + 16 * u + r16, a.N * G - 1), node = r / G;
@@ -216,8 +226,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
 #pragma unroll
       for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
       const uint64_t w = lane64(see, node);
-      sees[u] = near_nodes(w, a.window);
+      node_of[u] = w != 0;
       from[u] = a.window ? ct.len + __popcll(w) - a.window : 0;
+      // by the nodes' stage: its first `joint` keys are the context's last ones
+      const uint64_t ctx = ~0ull << min(max(from[u] - (ct.len - joint), 0), 63) & ((1ull << joint) - 1);  // joint is 63 at most
+      sees[u] = near_nodes(w, a.window) << joint | ctx;
     }
     f32x4 o[RT][DT];
     float m[RT], l[RT];
@@ -230,7 +243,8 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     const long head = ((long)b * a.Hkv + gh) * a.Smax * D;
     const bf16_t* const kc = (const bf16_t*)a.kc + head + (long)ct.lo * D;
     const bf16_t* const vc = (const bf16_t*)a.vc + head + (long)ct.lo * D;
-    const int full = (ct.len - ct.lo) / SK;  // stages of SK keys
+    const bf16_t* const nk = x + (long)(a.Hq + gh) * D;
+    const bf16_t* const nv = nk + (long)a.Hkv * D;
     constexpr int NJ = KB / 1024 / NW;       // this wave's loads of the keys' (values') image
     uint32_t off[2 * NJ];
     int key_of[NJ];
@@ -243,25 +257,36 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     }
     auto stage = [&](int tile, int buf) {
       char* const dst = smem + 2 * buf * KB + wid * 1024;
-      if (tile < full) {
+      if (tile < ct.full) {
         const long at = (long)tile * SK * D;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           paged::lds_dma16(kc + at, off[j], dst + j * NW * 1024);
           paged::lds_dma16(vc + at, off[NJ + j], dst + KB + j * NW * 1024);
         }
+        asm volatile("; a whole stage");
         return;
       }
       // keys behind the last one repeat it: they are masked, and what lies there is nobody's
+      const long at = (long)tile * SK * D;
       const bool own = tile == ct.tiles - 1;
-      const bf16_t* const kb = own ? x + (long)(a.Hq + gh) * D : kc + (long)tile * SK * D;
-      const bf16_t* const vb = own ? x + (long)(a.Hq + a.Hkv + gh) * D : vc + (long)tile * SK * D;
-      const int last = own ? n - 1 : ct.len - ct.lo - tile * SK - 1, pitch = own ? (int)a.ldq * 2 : D * 2;
+      const int ctx = own ? joint : ct.rest;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const int key = min(key_of[j], last) * pitch;
-        paged::lds_dma16(kb, (uint32_t)(key + (off[j] & (2 * D - 1))), dst + j * NW * 1024);
-        paged::lds_dma16(vb, (uint32_t)(key + (off[NJ + j] & (2 * D - 1))), dst + KB + j * NW * 1024);
+        const uint32_t ck = off[j] & (2 * D - 1), cv = off[NJ + j] & (2 * D - 1);
+        // the comments keep the compiler from joining loads of different bases, each of which would become a loop over the bases
+        if (!own || key_of[j] < ctx) {
+          const uint32_t key = min(key_of[j], ctx - 1) * (D * 2);
+          paged::lds_dma16(kc + at, key + ck, dst + j * NW * 1024);
+          paged::lds_dma16(vc + at, key + cv, dst + KB + j * NW * 1024);
+          asm volatile("; last keys of the context");
+        }
+        if (own && key_of[j] >= ctx) {
+          const uint32_t key = min(key_of[j] - ctx, n - 1) * (uint32_t)(a.ldq * 2);
+          paged::lds_dma16(nk, key + ck, dst + j * NW * 1024);
+          paged::lds_dma16(nv, key + cv, dst + KB + j * NW * 1024);
+          asm volatile("; nodes");
+        }
       }
     };
     if (tid < 2) bad[tid] = 0;
@@ -410,11 +435,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
       if constexpr (MODE == 2) {
         const uint64_t ill = ((uint64_t)bad[1] << 32 | bad[0]) & (KT == 64 ? ~0ull : 0xffffffffull << (wk * KT));
         for (uint64_t w = ill; w; w &= w - 1) {
-          const int node = __builtin_ctzll(w);
-          const bf16_t* const v = x + (long)node * a.ldq + (long)(a.Hq + a.Hkv + gh) * D + 4 * g;
+          const int key = __builtin_ctzll(w);
+          const bf16_t* const v = (key < joint ? vc + ((long)ct.full * SK + key) * D : nv + (long)(key - joint) * a.ldq) + 4 * g;
 #pragma unroll
           for (int u = 0; u < RT; ++u)
-            if (sees[u] >> node & 1)
+            if (sees[u] >> key & 1)
 #pragma unroll
               for (int c = 0; c < DT; ++c)
 #pragma unroll
@@ -428,7 +453,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     int t = t0;
     if (a.window)  // stages that the last nodes do not see all of
       for (; t < min(t1, ct.tiles - 1) && ct.lo + t * SK < ct.len + NODES - a.window; ++t) turn(std::integral_constant<int, 1>(), t);
-    for (; t < min(t1, full); ++t) turn(std::integral_constant<int, 0>(), t);
+    for (; t < min(t1, ct.full); ++t) turn(std::integral_constant<int, 0>(), t);
     for (; t < min(t1, ct.tiles - 1); ++t) turn(std::integral_constant<int, 1>(), t);
     if (t < t1) turn(std::integral_constant<int, 2>(), t);
 #pragma unroll
@@ -477,7 +502,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 4 * g;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
-          *(uint2*)(p + 16 * c) = sees[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
+          *(uint2*)(p + 16 * c) = node_of[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
                                           : make_uint2(0, 0);
       }
     }
@@ -505,6 +530,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
   float m = -INFINITY, l = 0.f;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
   int parts = a.S;
+  const int n = count_nodes(lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0);
   for (int s0 = 8 * w; s0 < parts; s0 += 8 * WAVES) {
     float2 ml[8];
     f32x4 po[8];
@@ -514,7 +540,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
       ml[k] = *(const float2*)(q + tiles * 16 * D + 2 * r);
       po[k] = ((const f32x4*)(q + 16 * tile * D))[64 * c + lane];
     }
-    parts = cut(a, b, SK).parts;
+    parts = cut(a, b, n, SK).parts;
     float mx = m;
 #pragma unroll
     for (int k = 0; k < 8; ++k)

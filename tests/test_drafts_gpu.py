@@ -93,6 +93,28 @@ def test_attention_window(Hq, Hkv, D, N, window):
     _attention(Hq, Hkv, D, N, [300, 20, 0, 101], 310, starts=[0, 4, 0, 50], window=window, junk=3.0)
 
 
+@pytest.mark.parametrize("window", [0, 3, 40])
+@pytest.mark.parametrize("N", [1, 31, 32, 63, 64])
+def test_attention_last_keys_beside_the_nodes(N, window):
+    """what is left of the context behind whole stages of 64 keys, beside the nodes, at and around the place where both fill a stage"""
+    lens = [n for rest in (0, 1, 63 - N, 64 - N, 65 - N, 63) for n in (rest, 64 + rest) if n >= 0]
+    _attention(4, 2, 64, N, lens, 200, window=window, junk=math.nan if not window else 5.0, starts=[n // 7 for n in lens] if N % 2 else None, seed=N)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_keeps_windows_apart(bad):
+    """a value that is no number at the end of the context reaches the nodes whose window holds it, and no other"""
+    N, window, n = 9, 4, 40  # node i at position n + i of a chain sees the slots from n + i - 3
+    qkv, kc, vc = _rand(N, 8 * 64), _rand(1, 2, 50, 64, seed=1), _rand(1, 2, 50, 64, seed=2)
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))]))
+    want = ops.tree_attention(qkv, kc, vc, _i32([n]), tree, 4, window=window)
+    vc[0, :, n - 2, 5] = bad
+    got = ops.tree_attention(qkv, kc, vc, _i32([n]), tree, 4, window=window)
+    assert torch.equal(got[2:], want[2:])
+    of = got[:2].view(2, 4, 64)
+    assert not torch.isfinite(of[:, :, 5]).any() and torch.isfinite(of[:, :, :5]).all()
+
+
 @pytest.mark.parametrize("lens", [[2100], [1500, 9, 700]])
 @pytest.mark.parametrize("N", [2, 30])
 def test_attention_long(lens, N):
