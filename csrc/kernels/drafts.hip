@@ -54,6 +54,7 @@ struct TreeArgs {
   void* o; long ldo;
   int B, N, Hq, Hkv, D, Smax, window;   // window 0: none
   float scale;
+  int G; float per_G;                   // Hq / Hkv and 1 / G
   int sorted, blocks;                   // long rows first; workgroups for a key head's rows
   float part_cost, join_cost;           // in stages
   float* part; int S;                   // partials of at most S shares of a row's keys (part_of)
@@ -166,10 +167,13 @@ __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int n, int SK) {
 }
 
 // a part of a pair's rows: of each 16 of them the accumulators as the lanes hold them [D / 16][64][4], behind all of these (m, l) of each row
-__device__ __forceinline__ int tiles16(const TreeArgs& a) { return (a.N * (a.Hq / a.Hkv) + 15) / 16; }
+__device__ __forceinline__ int tiles16(const TreeArgs& a) { return (a.N * a.G + 15) / 16; }
 __device__ __forceinline__ float* part_of(const TreeArgs& a, int D, int s, long pair) {
   return a.part + ((long)s * a.B * a.Hkv + pair) * ((long)tiles16(a) * 16 * (D + 2));
 }
+
+// r / G for a row r of a key head (under 64 G, G up to 4096: the error of the product is under 64 2^-23, and 1 / 2 G is more)
+__device__ __forceinline__ int node_of_row(const TreeArgs& a, int r) { return (int)((r + 0.5f) * a.per_G); }
 
 // ancestors less than `window` positions before a node: the last ones
 __device__ __forceinline__ uint64_t near_nodes(uint64_t see, int window) {
@@ -199,11 +203,19 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
   __shared__ unsigned bad[2];  // keys of the nodes' stage whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
-  // blocks go to the eight XCDs in turn: those that read the same keys for other rows come eight later, to the same L2
-  const int lin = a.blocks == 1 ? blockIdx.x : blockIdx.x / (8 * a.blocks) * 8 + blockIdx.x % 8, rb = a.blocks == 1 ? 0 : blockIdx.x / 8 % a.blocks;
-  const int s = lin % a.S, pair = lin / a.S;
-  if (pair >= a.B * a.Hkv) return;
-  const int b = a.sorted ? longest(a, pair / a.Hkv, lane) : pair / a.Hkv, gh = pair % a.Hkv, G = a.Hq / a.Hkv;
+  // (part, key head, row); where several workgroups share a key head's rows, the grid is (8 x these, all of the former by eight): blocks go to
+  // the eight XCDs in turn, and those that read the same keys come eight later, to the same L2
+  int s = blockIdx.x, gh = blockIdx.y, b = blockIdx.z, rb = 0;
+  if (a.blocks > 1) {
+    const int lin = blockIdx.y * 8 + (blockIdx.x & 7), pair = lin / a.S;
+    s = lin % a.S;
+    gh = pair % a.Hkv;
+    b = pair / a.Hkv;
+    rb = blockIdx.x >> 3;
+    if (b >= a.B) return;
+  }
+  if (a.sorted) b = longest(a, b, lane);
+  const int G = a.G;
   const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
   const int n = count_nodes(see), M = n * G;
   const Cut ct = cut(a, b, n, SK);
@@ -217,16 +229,16 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     bf16x8 qf[RT][DS];
     uint64_t sees[RT];
     int from[RT];  // first key of the context that the row sees
-    bool node_of[RT];
+    bool is_node[RT];
     const int joint = ct.tiles == ct.full + 1 ? ct.rest : 0;
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      const int r = min(row0 + 16 * u + r16, a.N * G - 1), node = r / G;
-      const bf16_t* const q = x + (long)node * a.ldq + (long)(gh * G + r % G) * D + 8 * g;
+      const int r = min(row0 + 16 * u + r16, a.N * G - 1), node = node_of_row(a, r);
+      const bf16_t* const q = x + (long)node * a.ldq + (long)(gh * G + r - node * G) * D + 8 * g;
 #pragma unroll
       for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
       const uint64_t w = lane64(see, node);
-      node_of[u] = w != 0;
+      is_node[u] = w != 0;
       from[u] = a.window ? ct.len + __popcll(w) - a.window : 0;
       // by the nodes' stage: its first `joint` keys are the context's last ones
       const uint64_t ctx = ~0ull << min(max(from[u] - (ct.len - joint), 0), 63) & ((1ull << joint) - 1);  // joint is 63 at most
@@ -499,10 +511,11 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         for (int c = 0; c < DT; ++c) q[64 * c] = o[u][c];
       } else if (r < M) {
         const float inv = 1.f / l[u];  // a node sees itself
-        bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 4 * g;
+        const int node = node_of_row(a, r);
+        bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + node) * a.ldo + (long)(gh * G + r - node * G) * D + 4 * g;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
-          *(uint2*)(p + 16 * c) = node_of[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
+          *(uint2*)(p + 16 * c) = is_node[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
                                           : make_uint2(0, 0);
       }
     }
@@ -521,7 +534,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
 template <int D, int WAVES>
 __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
   __shared__ float sh[4][6][64];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w = wid % WAVES, r16 = lane & 15, g = lane >> 4, G = a.Hq / a.Hkv;
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, w = wid % WAVES, r16 = lane & 15, g = lane >> 4, G = a.G;
   const int tiles = tiles16(a);
   const long all = (long)a.B * a.Hkv * tiles * (D / 16), id = (long)blockIdx.x * (4 / WAVES) + wid / WAVES, at = min(id, all - 1);
   const int c = (int)(at % (D / 16)), tile = (int)(at / (D / 16) % tiles);
@@ -665,9 +678,8 @@ template <int D, int RT, int WR, int WK, int KT>
 static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
   TreeArgs t = a;
   t.blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
-  const int all = a.S * a.B * a.Hkv;
-  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), dim3((unsigned)(t.blocks == 1 ? all : (all + 7) / 8 * 8 * t.blocks)), dim3(64 * WR * WK),
-                     0, stream, t);
+  const dim3 grid = t.blocks == 1 ? dim3(a.S, a.Hkv, a.B) : dim3(8 * t.blocks, (unsigned)(((long)a.S * a.B * a.Hkv + 7) / 8));
+  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), grid, dim3(64 * WR * WK), 0, stream, t);
 }
 template <int D>
 static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
@@ -701,7 +713,7 @@ static void tree_costs(int B, int N, int Hq, int Hkv, int D, float& part, float&
 // fill the CUs once; 1, and no second launch, where a full cache would not gain a quarter by them (the launch costs 3 us also where no
 // row turns out long enough).
 extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax, int window) {
-  if ((D != 64 && D != 128) || B == 0) return 0;
+  if ((D != 64 && D != 128) || B == 0 || Hq / Hkv > 4096 || (long)B * Hkv > 500000) return 0;  // grids
   const int rows = N * (Hq / Hkv), blocks = B * Hkv * (rows <= WIDE_ROWS ? (rows + 63) / 64 : (rows + 255) / 256);
   const int stages = ((window ? std::min(Smax, window) : Smax) + 63) / 64 + 1;
   const int most = std::max(1, std::min((num_cus() + blocks / 2) / blocks, stages));
@@ -716,7 +728,7 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
                                  int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, 0, 1, 0.f, 0.f, part, S};
+  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, Hq / Hkv, 1.f / (Hq / Hkv), 0, 1, 0.f, 0.f, part, S};
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
     if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
