@@ -39,13 +39,25 @@ void on(const Tensor& t, const Tensor& like, const char* n) {
 }
 void act(const Tensor& t, const char* n) {
   TORCH_CHECK_VALUE(t.is_cuda() && (t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat), n,
-              ": GPU tensor of bf16 or fp32 expected");
+                    ": GPU tensor of bf16 or fp32 expected");
 }
 bool al(const Tensor& t, uintptr_t n) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % n == 0; }
 void whole(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
   on(t, like, n);
   TORCH_CHECK_VALUE(t.scalar_type() == type && t.sizes() == shape && t.is_contiguous(), n, ": contiguous ", type, " ", shape, " expected, got ",
-              t.scalar_type(), " ", t.sizes());
+                    t.scalar_type(), " ", t.sizes());
+}
+
+// rows that share no element: other memory, or other columns of the same rows
+bool apart(const Tensor& a, const Tensor& b) {
+  if (!a.numel() || !b.numel() || !a.is_alias_of(b)) return true;
+  const int64_t size = a.element_size(), la = (a.size(0) - 1) * a.stride(0) + a.size(1), lb = (b.size(0) - 1) * b.stride(0) + b.size(1);
+  const char *pa = (const char*)a.data_ptr(), *pb = (const char*)b.data_ptr();
+  if (pa + la * size <= pb || pb + lb * size <= pa) return true;
+  const int64_t pitch = b.stride(0), bytes = pa - pb;
+  if (a.stride(0) != pitch || pitch == 0 || bytes % size) return false;
+  const int64_t col = ((bytes / size) % pitch + pitch) % pitch;  // a's first column, of b's
+  return col >= b.size(1) && col + a.size(1) <= pitch;
 }
 
 // whole numbers of a row each, contiguous
@@ -97,7 +109,8 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   on(out, qkv, "tree_attention out");
   TORCH_CHECK_VALUE(out.scalar_type() == qkv.scalar_type() && out.dim() == 2 && out.size(0) == B * N && out.size(1) == Hq * D &&
                         (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
-  at::assert_no_overlap(out, qkv);
+  at::assert_no_internal_overlap(out);
+  TORCH_CHECK_VALUE(apart(out, qkv), "tree_attention: out overlaps qkv");
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window) : 0;
   // matrix instructions want rows at 16 bytes (the output at 8): others are copied
@@ -119,6 +132,7 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
               "tree_accept: caches [layers, rows, heads, slots, dim] and rows of every layer (256 at most)");
   const int64_t L = kc.size(0), B = kc.size(1), Hkv = kc.size(2), Smax = kc.size(3), D = kc.size(4), N = see.size(1);
   on(vc, kc, "tree_accept v_cache");
+  TORCH_CHECK_VALUE(D > 0 && Hkv > 0, "tree_accept: caches of no heads");
   TORCH_CHECK_VALUE(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
               "tree_accept: caches of one type and layout, contiguous in each layer");
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
@@ -158,10 +172,10 @@ std::vector<Tensor> alternatives(const Tensor& logits, const optional<Tensor>& t
 }
 
 struct AlternativesFn : torch::autograd::Function<AlternativesFn> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const Tensor& targets, double c,
-                                                int64_t top) {
-    auto r = alternatives(logits, targets.defined() ? optional<Tensor>(targets) : c10::nullopt, c, top, true);
-    ctx->save_for_backward({logits, targets, r[3], r[4]});
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, const optional<Tensor>& targets,
+                                                double c, int64_t top) {
+    auto r = alternatives(logits, targets, c, top, true);
+    ctx->save_for_backward({logits, has(targets) ? *targets : Tensor(), r[3], r[4]});
     ctx->saved_data["c"] = c;
     ctx->mark_non_differentiable({r[3]});
     ctx->set_materialize_grads(false);
@@ -192,9 +206,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_alternatives(const Tensor& logi
   act(logits, "logits");
   TORCH_CHECK_VALUE(logits.dim() == 2 && top >= 1 && top <= 32 && top <= logits.size(1) && logits.size(1) < (1L << 30),
                     "1 to 32 alternatives of logits [tokens, vocabulary] expected: ", top, " of ", logits.sizes());
-  TORCH_CHECK_VALUE(c > 0 && std::isfinite((float)c), "inverse temperature ", c);
+  TORCH_CHECK_VALUE((float)c > 0 && std::isfinite((float)c), "inverse temperature ", c);
   const Tensor x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
-  Tensor t;
+  optional<Tensor> t;
   if (has(targets)) {
     on(*targets, logits, "targets");
     TORCH_CHECK_VALUE(targets->dim() == 1 && targets->size(0) == logits.size(0) && at::isIntegralType(targets->scalar_type(), false),
@@ -202,7 +216,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_alternatives(const Tensor& logi
     t = targets->to(at::kLong).contiguous();
   }
   auto r = at::GradMode::is_enabled() && x.requires_grad() ? AlternativesFn::apply(x, t, c, top)
-                                                            : alternatives(x, t.defined() ? optional<Tensor>(t) : c10::nullopt, c, top, false);
+                                                            : alternatives(x, t, c, top, false);
   return {r[0], r[1], r[2], r[3]};
 }
 

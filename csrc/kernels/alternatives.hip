@@ -78,15 +78,16 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // The alternatives without sorting: the best of each lane's elements over the waves makes 64 numbers of which no two are equal (value,
 // then place), and the top-th of them is one that at least `top` elements reach. What reaches it is a little more than `top` elements (24 of 32000
 // where 20 are wanted); each counts how many of the others are before it. Where they are more than CAP (rows made for it) the
-// best are taken one by one.
+// best are taken one by one. Bound by memory with many rows (4096 x 32000 in bf16: 56 us, 4.7 TB/s), by the exp of one CU's row and a chain of
+// barriers with few (8 rows: 8 us).
 template <typename T, int THREADS, int NC>
-__global__ __launch_bounds__(THREADS, NC ? 1 : 8) void alternatives_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
-                                                               int V, int top, float* __restrict__ logp, float* __restrict__ ent,
-                                                               float* __restrict__ top_lp, int64_t* __restrict__ ids,
-                                                               float* __restrict__ stats) {
-  constexpr int E = Chunk<T>::E, NW = THREADS / 64, KEEP = NC ? NC : 1;
+__global__ __launch_bounds__(THREADS, NC ? 1 : 8) void alternatives_kernel(const T* __restrict__ logits, long ld,
+                                                                           const int64_t* __restrict__ tgt, float c, int V, int top,
+                                                                           float* __restrict__ logp, float* __restrict__ ent,
+                                                                           float* __restrict__ top_lp, int64_t* __restrict__ ids,
+                                                                           float* __restrict__ stats) {
+  constexpr int E = Chunk<T>::E, NW = THREADS / 64, KEEP = NC ? NC : 1, SHARE = 64 / NW;
   __shared__ float sm[3][NW];
-  constexpr int SHARE = 64 / NW;
   __shared__ uint64_t best[THREADS], cand[CAP], group[64], tau_s;
   __shared__ int ahead[NW][64];
   __shared__ int count;
@@ -231,7 +232,8 @@ __global__ __launch_bounds__(THREADS, NC ? 1 : 8) void alternatives_kernel(const
     unsigned hits = 0;
     const int q = tch >= tid ? (tch - tid) / THREADS : -1;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) if (k * THREADS < chunks) hits |= (top_of[k] > tv || (top_of[k] == tv && k <= q) ? 1u : 0u) << k;
+    for (int k = 0; k < NC; ++k)
+      if (k * THREADS < chunks) hits |= (top_of[k] > tv || (top_of[k] == tv && k <= q) ? 1u : 0u) << k;
     for (; hits; hits &= hits - 1) {
       const int ch = __builtin_ctz(hits) * THREADS + tid;
       if (ch < chunks) look(ch, load_chunk(x, ch, V));
@@ -284,7 +286,8 @@ __global__ __launch_bounds__(THREADS, NC ? 1 : 8) void alternatives_kernel(const
 }
 
 // dl = c (up - p (sum up) - g_H p (z - mean)), up: the given token's and the alternatives' gradients at their places. A row is read and
-// written once; the places with gradients of their own, 33 at most, are written again behind the chunks that hold them.
+// written once; the places with gradients of their own, 33 at most, are written again behind the chunks that hold them. Bound by
+// memory (2048 x 32002 in bf16: 44 us, 6 TB/s read and written, part of it from the cache that the forward filled).
 template <typename T>
 __global__ __launch_bounds__(256) void alternatives_bwd_kernel(const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float c,
                                                                int V, int top, const int64_t* __restrict__ ids,
@@ -376,7 +379,9 @@ static int launch_alternatives(const T* x, long ld, const int64_t* tgt, float c,
 #define ALT(THREADS, NC)                                                                                                                 \
   hipLaunchKernelGGL((alternatives_kernel<T, THREADS, NC>), dim3((unsigned)rows), dim3(THREADS), 0, stream, x, ld, tgt, c, V, top, logp, ent, \
                      top_lp, ids, stats)
-  const bool few = rows <= num_cus();  // a row a CU: as many threads as the row feeds
+  // up to a row a CU as many threads as the row feeds (8 rows of 32000 in bf16 8.9 us, with 256 threads 9.6); beyond, rows of 256 and 512 threads that
+  // share a CU and wait at different times (300 rows 14.3 us, with 1024 threads 17.1; 1000 rows 22.6 and 35)
+  const bool few = rows <= num_cus();
   if (chunks <= 256 * 4) ALT(256, 4);
   else if (few && chunks <= 1024 * 4) ALT(1024, 4);
   else if (!few && chunks <= 256 * 16) ALT(256, 16);
@@ -401,7 +406,7 @@ template <typename T>
 static int launch_alternatives_bwd(const T* x, long ld, const int64_t* tgt, float c, long rows, int V, int top, const int64_t* ids,
                                    const float* stats, const float* g_lp, const float* g_ent, const float* g_top, T* d, long ldd,
                                    hipStream_t stream) {
-  // a row goes to several workgroups where rows are few: eight of them a CU, with four chunks a thread at least
+  // a row goes to several workgroups where rows are few: eight of them a CU, with four chunks a thread at least (333 x 50272 in fp32 72 -> 28 us)
   const int chunks = (V + Chunk<T>::E - 1) / Chunk<T>::E;
   const int parts = (int)std::max(1L, std::min((8L * num_cus() + rows - 1) / rows, (long)(chunks + 1023) / 1024));
   const int span = ((chunks + parts - 1) / parts + 255) / 256 * 256;

@@ -494,7 +494,6 @@ class CausalLM(nn.Module):
             x, residual = layer.mlp(o, residual)
         return self.final_norm(x, residual), drafts
 
-
     # ------------------------------------------------------------------ LoRA
     def add_lora(self, r: int = 16, alpha: float = 32.0, targets=None, dropout: float = 0.0, seed: int = 0):
         """Attach PEFT-style LoRA adapters (A kaiming-uniform, B zero) to the target projections."""

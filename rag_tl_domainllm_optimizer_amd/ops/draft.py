@@ -59,7 +59,7 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of drafted tokens -> [rows * nodes, Hq * D]. ``qkv`` [rows * nodes, >= (Hq + 2 Hkv) * D] holds the nodes' rotated rows [q | k | v];
     node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
     key; with ``window`` only those less than ``window`` positions before it. Nothing is appended to the caches; rows that are not
-    nodes come out as zeros. What other nodes hold, NaN among it, does not reach a node."""
+    nodes come out as zeros. ``out`` may be columns of wider rows, but shares nothing with ``qkv``. What other nodes hold, NaN among it, does not reach a node."""
     if on_gpu(qkv):
         return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
@@ -99,6 +99,8 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
         raise ValueError(f"tree {tuple(tree.shape)}, tokens {tuple(tokens.shape)} and choice {tuple(choice.shape)} of {B} rows do not go together")
     if tokens.dtype != torch.int64 or choice.dtype != torch.int64:
         raise ValueError("tokens and choice: int64 expected")
+    if D < 1 or Hkv < 1:
+        raise ValueError("caches of no heads")
     if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or x.dtype != k_cache.dtype or x.shape[0] != B * tree.shape[1]
                                or x.shape[1] % D or x.shape[1] <= 2 * Hkv * D for x in drafts):
         raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")

@@ -153,8 +153,9 @@ def token_logprobs(logits: torch.Tensor, targets, inv_temp: float = 1.0):
 def token_alternatives(logits: torch.Tensor, targets, top: int, inv_temp: float = 1.0):
     """:func:`token_logprobs` with the best alternatives: logits [T, V] (bf16 or fp32; rows may be strided) -> (log p(target) [T], entropy [T], the
     log-probabilities of the ``top`` (1 to 32) most likely tokens, best first [T, top], their ids int64 [T, top]) of softmax(logits * inv_temp),
-    all but the ids differentiable. Targets below 0, or None, have log-probability 0; a target from V on has NaN on a GPU. Equally likely tokens go by their id and a NaN logit counts as the least likely; a row of -inf alone has log-probabilities
-    of -inf, entropy 0 and no gradient."""
+    all but the ids differentiable (once). Targets below 0, or None, have log-probability 0; a target from V on has NaN on a GPU. Equally likely
+    tokens go by their id, and a NaN logit counts as the least likely; a row of -inf alone has log-probabilities of -inf, entropy 0 and
+    no gradient."""
     if on_gpu(logits):
         return native().token_alternatives(logits, targets, top, inv_temp)
     if logits.dim() != 2 or not 1 <= top <= min(32, logits.shape[1]):

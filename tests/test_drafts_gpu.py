@@ -143,6 +143,15 @@ def test_attention_into_columns_of_a_wider_output():
         assert (wide[:, :at] == 5).all() and (wide[:, at + Hq * D:] == 5).all()
 
 
+def test_attention_into_other_columns_of_the_same_rows():
+    B, N, Hq, Hkv, D = 2, 5, 4, 2, 64
+    wide = _rand(B * N, (Hq + 2 * Hkv) * D + Hq * D)
+    qkv, kc, vc = wide[:, :(Hq + 2 * Hkv) * D], _rand(B, Hkv, 50, D, seed=1), _rand(B, Hkv, 50, D, seed=2)
+    tree, lens = ops.draft_tree(_i32(plain.trees(B, N, 0))), _i32([50, 20])
+    want = ops.tree_attention(qkv.clone(), kc, vc, lens, tree, Hq)
+    assert torch.equal(ops.tree_attention(qkv, kc, vc, lens, tree, Hq, out=wide[:, (Hq + 2 * Hkv) * D:]), want)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (4, 4, 64), (3, 1, 32)])
 def test_attention_keeps_nodes_apart(Hq, Hkv, D, bad):
@@ -354,6 +363,19 @@ def test_alternatives_of_strided_rows(pitch, at, dtype):
     _check_alternatives(wide.t()[:6].t().contiguous().t()[:, :6], torch.zeros(6, dtype=torch.int32, device=DEV), 2, 1.0)
 
 
+def test_alternatives_without_targets():
+    _check_alternatives(_rand(5, 300, dtype=F32, seed=1), None, 7, 1.0)
+
+
+def test_alternatives_offsets_past_32_bits():
+    """rows 2^30 + 5 elements apart: the last one lies behind 2^31 elements and 2^32 bytes"""
+    V, pitch = 1000, 2 ** 30 + 5
+    store = torch.empty(2 * pitch + V, dtype=BF16, device=DEV)
+    x = store.as_strided((3, V), (pitch, 1))
+    x.copy_(_rand(3, V, seed=1))
+    _check_alternatives(x, torch.tensor([0, 999, 500], device=DEV), 5, 1.0)
+
+
 def test_alternatives_nothing_to_do():
     x = torch.zeros(0, 100, dtype=BF16, device=DEV, requires_grad=True)
     lp, ent, top, ids = ops.token_alternatives(x, torch.zeros(0, dtype=torch.long, device=DEV), 3)
@@ -521,7 +543,13 @@ def test_runs_repeat_bit_by_bit():
     lambda: ops.tree_attention(_rand(2, 512), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, scale=-1.0),
     lambda: ops.tree_attention(_rand(2, 512), *(torch.zeros(1, 2, 9, 64, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4),
     lambda: ops.draft_tree(torch.zeros(2, 65, dtype=torch.int32, device=DEV)),
+    lambda: ops.tree_attention(_rand(2, 512), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4,
+                               out=torch.empty(1, 256, dtype=BF16, device=DEV).expand(2, 256)),
+    lambda: _in_place(_rand(2, 512)),
+    lambda: ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.long, device=DEV) for _ in "tc"), [_rand(2, 512)],
+                            *(torch.zeros(1, 1, 2, 9, 0, dtype=BF16, device=DEV) for _ in "kv"), _i32([3])),
     lambda: ops.token_alternatives(_rand(2, 50), None, 33),
+    lambda: ops.token_alternatives(_rand(2, 50), None, 2, 1e-60),
     lambda: ops.token_alternatives(_rand(2, 50), None, 2, math.inf),
     lambda: ops.token_alternatives(_rand(2, 50), torch.zeros(3, dtype=torch.long, device=DEV), 2),
     lambda: ops.token_alternatives(_rand(2, 50).half(), None, 2),
@@ -530,6 +558,10 @@ def test_runs_repeat_bit_by_bit():
 def test_refused(bad):
     with pytest.raises((ValueError, RuntimeError)):
         bad()
+
+
+def _in_place(qkv):
+    return ops.tree_attention(qkv, _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, out=qkv[:, :256])
 
 
 def test_a_model_checks_drafts_like_single_steps():
