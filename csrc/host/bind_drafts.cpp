@@ -6,6 +6,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <tuple>
 #include <vector>
@@ -13,10 +14,10 @@
 extern "C" {
 int rt_draft_tree(const int*, const int*, const int*, int, int, int64_t*, int*, hipStream_t);
 int rt_tree_parts(int, int, int, int, int, int, int);
-int rt_tree_attention(int, const void*, long, const void*, const void*, const int*, const int*, const int64_t*, void*, long, float*, int, int,
-                      int, int, int, int, int, int, float, hipStream_t);
+int rt_tree_attention(int, const void*, long, const void*, const void*, const float*, const float*, int, const int*, const int*, const int64_t*,
+                      void*, long, float*, int, int, int, int, int, int, int, int, float, hipStream_t);
 int rt_tree_accept(const int*, const int64_t*, const int64_t*, const int64_t*, const int*, int*, int*, int64_t*, const void* const*, long, void*,
-                   void*, long, int, int, int, int, int, int, int, int, hipStream_t);
+                   void*, long, float*, float*, long, int, int, int, int, int, int, int, int, int, hipStream_t);
 int rt_alternatives(int, const void*, long, const int64_t*, float, long, int, int, float*, float*, float*, int64_t*, float*, hipStream_t);
 int rt_alternatives_bwd(int, const void*, long, const int64_t*, float, long, int, int, const int64_t*, const float*, const float*, const float*,
                         const float*, void*, long, hipStream_t);
@@ -60,6 +61,28 @@ bool apart(const Tensor& a, const Tensor& b) {
   return col >= b.size(1) && col + a.size(1) <= pitch;
 }
 
+// the slots' scales of an e4m3 cache [.., rows, heads, slots, 128], alike for keys and values
+struct Scales { float* k = nullptr; float* v = nullptr; long layer = 0; int slots = 0; };
+Scales scales(const Tensor& kc, const optional<Tensor>& k, const optional<Tensor>& v) {
+  Scales r;
+  TORCH_CHECK_VALUE(has(k) == has(v), "scales of keys and values go together");
+  TORCH_CHECK_VALUE(has(k) == (kc.scalar_type() == at::kByte), "scales belong to an e4m3 cache (uint8), and it has them");
+  if (!has(k)) return r;
+  const int64_t n = kc.dim();
+  for (const auto* t : {&*k, &*v}) {
+    on(*t, kc, "scales");
+    TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == n - 1 && t->sizes().slice(0, n - 2) == kc.sizes().slice(0, n - 2) &&
+                          t->size(n - 2) >= kc.size(n - 2) && (n == 4 ? *t : t->select(0, 0)).is_contiguous() && t->sizes() == k->sizes() &&
+                          t->strides() == k->strides(), "scales: fp32 of every row, head and slot expected, got ", t->sizes());
+  }
+  TORCH_CHECK_VALUE(kc.size(n - 1) == 128, "an e4m3 cache has heads of 128");
+  r.k = k->data_ptr<float>();
+  r.v = v->data_ptr<float>();
+  r.layer = k->stride(0);
+  r.slots = (int)k->size(n - 2);
+  return r;
+}
+
 // whole numbers of a row each, contiguous
 Tensor ints(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Tensor& like, const char* n) {
   on(t, like, n);
@@ -85,15 +108,17 @@ std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parent_, const optio
 }
 
 Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& kv_len_, const optional<Tensor>& kv_start_,
-                      const Tensor& see, const optional<Tensor>& out_, int64_t Hq, int64_t window, const optional<double>& scale_) {
+                      const Tensor& see, const optional<Tensor>& out_, int64_t Hq, int64_t window, const optional<double>& scale_,
+                      const optional<Tensor>& k_scale, const optional<Tensor>& v_scale) {
   act(qkv, "tree_attention qkv");
   TORCH_CHECK_VALUE(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && (qkv.stride(1) == 1 || qkv.size(0) == 0),
                     "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim] expected, got ", qkv.sizes(), ", ", kc.sizes());
   const int64_t B = kc.size(0), Hkv = kc.size(1), Smax = kc.size(2), D = kc.size(3), N = see.size(1);
-  TORCH_CHECK_VALUE(kc.scalar_type() == qkv.scalar_type(), "caches of ", kc.scalar_type(), " under queries of ", qkv.scalar_type(),
-                    ": an fp8 cache is read by decode_step_attention only");
-  whole(kc, qkv.scalar_type(), kc.sizes(), qkv, "tree_attention k_cache");
-  whole(vc, qkv.scalar_type(), kc.sizes(), qkv, "tree_attention v_cache");
+  const Scales sc = scales(kc, k_scale, v_scale);
+  TORCH_CHECK_VALUE(sc.k ? qkv.scalar_type() == at::kBFloat16 : kc.scalar_type() == qkv.scalar_type(), "caches of ", kc.scalar_type(),
+                    " under queries of ", qkv.scalar_type());
+  whole(kc, kc.scalar_type(), kc.sizes(), qkv, "tree_attention k_cache");
+  whole(vc, kc.scalar_type(), kc.sizes(), qkv, "tree_attention v_cache");
   whole(see, at::kLong, {B, N}, qkv, "tree_attention tree");
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, qkv, "kv_len");
   const optional<Tensor> kv_start = ints(kv_start_, at::kInt, {B}, qkv, "kv_start");
@@ -113,21 +138,24 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   TORCH_CHECK_VALUE(apart(out, qkv), "tree_attention: out overlaps qkv");
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window) : 0;
+  TORCH_CHECK_VALUE(S || !sc.k || !B, "tree_attention: an e4m3 cache of this size");
   // matrix instructions want rows at 16 bytes (the output at 8): others are copied
   Tensor x = qkv, o = out;
   if (S && !(al(x, 16) && x.stride(0) % 8 == 0 && x.stride(0) < (1L << 24))) x = qkv.narrow(1, 0, (Hq + 2 * Hkv) * D).clone(at::MemoryFormat::Contiguous);
   if (S && !(al(o, 8) && o.stride(0) % 4 == 0)) o = at::empty({B * N, Hq * D}, qkv.options());
   Tensor part = S > 1 ? at::empty({S * B * Hkv * ((N * (Hq / Hkv) + 15) / 16) * 16 * (D + 2)}, qkv.options().dtype(at::kFloat)) : Tensor();
-  rc_ok(rt_tree_attention(x.scalar_type() == at::kFloat, x.data_ptr(), x.stride(0), kc.data_ptr(), vc.data_ptr(), kv_len.data_ptr<int>(),
-                          ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
+  rc_ok(rt_tree_attention(x.scalar_type() == at::kFloat, x.data_ptr(), x.stride(0), kc.data_ptr(), vc.data_ptr(), sc.k, sc.v, sc.slots,
+                          kv_len.data_ptr<int>(), ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
                           (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, stream()), "tree_attention");
   if (!o.is_same(out)) out.copy_(o);
   return out;
 }
 
 std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens_, const Tensor& choice_,
-                                               const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len_) {
-  act(kc, "tree_accept k_cache");
+                                               const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len_,
+                                               const optional<Tensor>& k_scale, const optional<Tensor>& v_scale) {
+  if (!has(k_scale)) act(kc, "tree_accept k_cache");
+  TORCH_CHECK_VALUE(kc.is_cuda(), "tree_accept k_cache: GPU tensor expected");
   TORCH_CHECK_VALUE(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
               "tree_accept: caches [layers, rows, heads, slots, dim] and rows of every layer (256 at most)");
   const int64_t L = kc.size(0), B = kc.size(1), Hkv = kc.size(2), Smax = kc.size(3), D = kc.size(4), N = see.size(1);
@@ -135,25 +163,31 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
   TORCH_CHECK_VALUE(D > 0 && Hkv > 0, "tree_accept: caches of no heads");
   TORCH_CHECK_VALUE(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
               "tree_accept: caches of one type and layout, contiguous in each layer");
+  const Scales sc = scales(kc, k_scale, v_scale);
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
   whole(see, at::kLong, {B, N}, kc, "tree_accept tree");
   const Tensor tokens = ints(tokens_, at::kLong, {B, N}, kc, "tokens"), choice = ints(choice_, at::kLong, {B, N}, kc, "choice");
   std::vector<const void*> at;
-  for (const Tensor& x : drafts) {
+  std::vector<Tensor> held;  // e4m3: rows at 16 bytes, others are copied
+  const bool copy = sc.k && std::any_of(drafts.begin(), drafts.end(), [](const Tensor& x) { return x.dim() != 2 || !al(x, 16) || x.stride(0) % 8; });
+  if (copy)
+    for (const Tensor& x : drafts) held.push_back(x.clone(at::MemoryFormat::Contiguous));
+  const std::vector<Tensor>& rows = copy ? held : drafts;
+  for (const Tensor& x : rows) {
     on(x, kc, "tree_accept drafts");
-    TORCH_CHECK_VALUE(x.scalar_type() == kc.scalar_type() && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
-                    x.stride(0) == drafts[0].stride(0) && x.size(0) == B * N && x.size(1) % D == 0 && x.size(1) / D > 2 * Hkv,
+    TORCH_CHECK_VALUE(x.scalar_type() == (sc.k ? at::kBFloat16 : kc.scalar_type()) && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == rows[0].sizes() &&
+                    x.stride(0) == rows[0].stride(0) && x.size(0) == B * N && x.size(1) % D == 0 && x.size(1) / D > 2 * Hkv,
                 "tree_accept: drafts [rows nodes, (heads + 2 key heads) dim] of the caches' type, alike in every layer");
     at.push_back(x.data_ptr());
   }
-  const int64_t Hq = drafts[0].size(1) / D - 2 * Hkv;
+  const int64_t Hq = rows[0].size(1) / D - 2 * Hkv;
   TORCH_CHECK_VALUE(N * Hkv * D < (1L << 30), "tree_accept: sizes");
   const c10::DeviceGuard guard(kc.device());
   Tensor count = at::empty({B}, parent.options()), path = at::empty({B, N}, parent.options()), next = at::empty({B}, tokens.options());
   rc_ok(rt_tree_accept(parent.data_ptr<int>(), see.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), choice.data_ptr<int64_t>(),
                        kv_len.data_ptr<int>(), count.data_ptr<int>(), path.data_ptr<int>(), next.data_ptr<int64_t>(), at.data(),
-                       drafts[0].stride(0), kc.data_ptr(), vc.data_ptr(), kc.stride(0), (int)B, (int)N, (int)L, (int)Hq, (int)Hkv, (int)Smax, (int)D,
+                       rows[0].stride(0), kc.data_ptr(), vc.data_ptr(), kc.stride(0), sc.k, sc.v, sc.layer, sc.slots, (int)B, (int)N, (int)L, (int)Hq, (int)Hkv, (int)Smax, (int)D,
                        (int)kc.element_size(), stream()), "tree_accept");
   return {count, path, next};
 }

@@ -49,6 +49,7 @@ __global__ __launch_bounds__(64) void draft_tree_kernel(const int* __restrict__ 
 struct TreeArgs {
   const void* qkv; long ldq;            // [B N, (Hq + 2 Hkv) D] rotated rows of the nodes
   const void* kc; const void* vc;       // [B, Hkv, Smax, D]
+  const float* ksc; const float* vsc; int SmaxP;  // scales [B, Hkv, SmaxP] of caches in e4m3 (keys' bytes in the order that decoding reads), or null
   const int* kv_len; const int* kv_start;
   const int64_t* see;                   // [B, N]
   void* o; long ldo;
@@ -150,7 +151,7 @@ __device__ __forceinline__ int count_nodes(uint64_t see) {
   return live ? 64 - __builtin_clzll(live) : 0;
 }
 
-// full: stages that the context fills; rest: its last keys, which go into the nodes' stage where both fit there
+// full: stages that the context fills; rest: its last keys, which go into the nodes' stage where both fit there (and are of one type)
 struct Cut { int lo, len, full, rest, tiles, parts, per; };
 __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int n, int SK) {
   Cut c;
@@ -160,7 +161,7 @@ __device__ __forceinline__ Cut cut(const TreeArgs& a, int b, int n, int SK) {
   c.lo = min(c.lo, c.len);
   c.full = (c.len - c.lo) / SK;
   c.rest = (c.len - c.lo) % SK;
-  c.tiles = c.full + (c.rest + n > SK ? 2 : 1);
+  c.tiles = c.full + (c.rest > (a.ksc ? 0 : SK - n) ? 2 : 1);
   c.per = stages_per_part(c.tiles, a.S, a.part_cost, a.join_cost);
   c.parts = (c.tiles + c.per - 1) / c.per;
   return c;
@@ -196,11 +197,12 @@ __device__ __forceinline__ int longest(const TreeArgs& a, int q, int lane) {
 // one v_maximum3_f32 for two of these; fmaxf has each operand made canonical first. A NaN stays one.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-template <int D, int RT, int WR, int WK, int KT>
+template <int D, int RT, int WR, int WK, int KT, bool KV8>
 __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
-  static_assert(KB / 1024 % NW == 0 && SK >= NODES);
+  static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
+  __shared__ __attribute__((aligned(16))) float scales[KV8 ? 2 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
   __shared__ unsigned bad[2];  // keys of the nodes' stage whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   // (part, key head, row); where several workgroups share a key head's rows, the grid is (8 x these, all of the former by eight): blocks go to
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     uint64_t sees[RT];
     int from[RT];  // first key of the context that the row sees
     bool is_node[RT];
-    const int joint = ct.tiles == ct.full + 1 ? ct.rest : 0;
+    const int joint = !KV8 && ct.tiles == ct.full + 1 ? ct.rest : 0;
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
       const int r = min(row0 + 16 * u + r16, a.N * G - 1), node = node_of_row(a, r);
@@ -269,7 +271,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     }
     auto stage = [&](int tile, int buf) {
       char* const dst = smem + 2 * buf * KB + wid * 1024;
-      if (tile < ct.full) {
+      if (!KV8 && tile < ct.full) {
         const long at = (long)tile * SK * D;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
       for (int j = 0; j < NJ; ++j) {
         const uint32_t ck = off[j] & (2 * D - 1), cv = off[NJ + j] & (2 * D - 1);
         // the comments keep the compiler from joining loads of different bases, each of which would become a loop over the bases
-        if (!own || key_of[j] < ctx) {
+        if (!KV8 && (!own || key_of[j] < ctx)) {
           const uint32_t key = min(key_of[j], ctx - 1) * (D * 2);
           paged::lds_dma16(kc + at, key + ck, dst + j * NW * 1024);
           paged::lds_dma16(vc + at, key + cv, dst + KB + j * NW * 1024);
@@ -301,36 +303,49 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         }
       }
     };
-    if (tid < 2) bad[tid] = 0;
-    stage(t0, 0);
-    int cur = 0;
-    // one stage; MODE 0: every row sees all of its keys, 1: some keys of the context are not seen, 2: the nodes' own keys
-    auto turn = [&](auto mode, int t) {
-      constexpr int MODE = decltype(mode)::value;
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
-      asm volatile("s_barrier" ::: "memory");                      // ... by every wave; the other buffer is free
-      if (MODE != 2 && t + 1 < t1) stage(t + 1, cur ^ 1);
-      char* const Ks = smem + 2 * cur * KB + wk * KT * D * 2;
-      char* const Vs = smem + (2 * cur + 1) * KB + wk * KT * D * 2;
-      if constexpr (MODE == 2) {
-        // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
-        // product and are added below for the rows that see them
-        char* const img = smem + (2 * cur + 1) * KB;
-        for (int e = tid; e < NODES * NC; e += 64 * NW) {
-          uint32_t* const w = (uint32_t*)(img + e * 16);
+    // a stage of an e4m3 cache: to registers while the stage before is multiplied, then as bf16 (exact) to LDS
+    constexpr int NU = KV8 ? SK * D / 16 / (64 * NW) : 1;
+    uint4 rk[NU], rv[NU];
+    float rs = 0.f;
+    auto fetch = [&](int tile) {
+      const long at = head + ((long)ct.lo + (long)tile * SK) * D;
+      const int last = ct.len - ct.lo - tile * SK - 1;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
-            if (lo || hi) {
-              w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
-              atomicOr(&bad[e / NC / 32], 1u << (e / NC % 32));
-            }
-          }
-        }
-        __syncthreads();
+      for (int j = 0; j < NU; ++j) {
+        const int e = j * 64 * NW + tid;
+        const long from = at + min(e / 8, last) * D + e % 8 * 16;
+        rk[j] = *(const uint4*)((const char*)a.kc + from);
+        rv[j] = *(const uint4*)((const char*)a.vc + from);
       }
-      cur ^= 1;
-      if (row0 >= M) return;
+      if (tid < 2 * SK) rs = (tid < SK ? a.ksc : a.vsc)[pair_at * a.SmaxP + ct.lo + tile * SK + min(tid % SK, last)];
+    };
+    auto settle = [&](int buf) {
+      char* const img = smem + 2 * buf * KB;
+#pragma unroll
+      for (int j = 0; j < NU; ++j) {
+        // 16 bytes h of a key: elements 8 (4 s + h / 2) .. + 7 of s = 2 (h % 2) and the next; of a value 16 h .. 16 h + 15
+        const int e = j * 64 * NW + tid, key = e / 8, h = e % 8, c = 8 * (h % 2) + h / 2;
+        *(bf16x8*)(img + paged::kq_off<D>(key, c)) = fp8x8_to_bf16(rk[j].x, rk[j].y);
+        *(bf16x8*)(img + paged::kq_off<D>(key, c + 4)) = fp8x8_to_bf16(rk[j].z, rk[j].w);
+        *(bf16x8*)(img + KB + paged::vv_off<D>(key, 2 * h)) = fp8x8_to_bf16(rv[j].x, rv[j].y);
+        *(bf16x8*)(img + KB + paged::vv_off<D>(key, 2 * h + 1)) = fp8x8_to_bf16(rv[j].z, rv[j].w);
+      }
+      if (tid < 2 * SK) scales[buf][tid] = rs;
+    };
+    if (tid < 2) bad[tid] = 0;
+    if (KV8 && t0 < ct.tiles - 1) {
+      fetch(t0);
+      settle(0);
+    } else {
+      stage(t0, 0);
+    }
+    int cur = 0;
+    // a stage that lies in LDS; MODE 0: every row sees all of its keys, 1: some keys of the context are not seen, 2: the nodes' own keys
+    auto multiply = [&](auto mode, int t, int now) {
+      constexpr int MODE = decltype(mode)::value;
+      constexpr bool SCALED = KV8 && MODE != 2;
+      char* const Ks = smem + 2 * now * KB + wk * KT * D * 2;
+      char* const Vs = smem + (2 * now + 1) * KB + wk * KT * D * 2;
       f32x4 st[KS][RT];
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -346,6 +361,16 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
           for (int u = 0; u < RT; ++u) st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][d], st[k][u], 0, 0, 0);
         }
       const int key0 = wk * KT + 4 * g;  // of the stage: this lane's keys are key0 + 16 k + e
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const f32x4 sc = *(const f32x4*)&scales[now][key0 + 16 * k];
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[k][u][e] *= sc[e];
+        }
+      }
       if constexpr (MODE == 2) {
 #pragma unroll
         for (int u = 0; u < RT; ++u)
@@ -410,6 +435,16 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
           }
         l[u] += sum;  // of this lane's keys; the four lanes are added at the end
       }
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const f32x4 sc = *(const f32x4*)&scales[now][SK + key0 + 16 * k];
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) st[k][u][e] *= sc[e];
+        }
+      }
       bf16x8 pf[KT / 32][RT];
 #pragma unroll
       for (int k = 0; k < KT / 32; ++k)
@@ -461,6 +496,35 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
                 }
         }
       }
+    };
+    auto turn = [&](auto mode, int t) {
+      constexpr int MODE = decltype(mode)::value;
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
+      asm volatile("s_barrier" ::: "memory");                      // ... by every wave; the other buffer is free
+      const bool more = MODE != 2 && t + 1 < t1, more8 = KV8 && more && t + 1 < ct.tiles - 1;
+      if (more8) fetch(t + 1);
+      else if (more) stage(t + 1, cur ^ 1);
+      const int now = cur;
+      cur ^= 1;
+      if constexpr (MODE == 2) {
+        // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
+        // product and are added below for the rows that see them
+        char* const img = smem + (2 * now + 1) * KB;
+        for (int e = tid; e < NODES * NC; e += 64 * NW) {
+          uint32_t* const w = (uint32_t*)(img + e * 16);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
+            if (lo || hi) {
+              w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
+              atomicOr(&bad[e / NC / 32], 1u << (e / NC % 32));
+            }
+          }
+        }
+        __syncthreads();
+      }
+      if (row0 < M) multiply(mode, t, now);
+      if (more8) settle(cur);
     };
     int t = t0;
     if (a.window)  // stages that the last nodes do not see all of
@@ -609,11 +673,13 @@ struct AcceptArgs {
   int* count; int* path; int64_t* next;
   void* kc; void* vc;                   // [L, B, Hkv, Smax, D], layers `layer` units apart
   long ldq, layer;
+  float* ksc; float* vsc; long sc_layer; int SmaxP;  // scales [L, B, Hkv, SmaxP] of e4m3 caches, or null
   int B, N, L, Hq, Hkv, Smax, row;      // row: 16-byte (or single element) units of a head's row
   const void* drafts[LAYERS];           // [B N, (Hq + 2 Hkv) D] of every layer
 };
 
-template <typename U>
+// KV8: rows of 128 in bf16 to e4m3 with a scale each, rounded and ordered as a prompt's are
+template <typename U, bool KV8>
 __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
   __shared__ int path[NODES];
   __shared__ int steps;
@@ -648,6 +714,26 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
   __syncthreads();
   const int len = max(a.kv_len[b], 0), n = min(steps, a.Smax - len);  // slots that are there
   const U* const x = (const U*)a.drafts[layer] + at * a.ldq;
+  if constexpr (KV8) {
+    const int c = tid & 15;  // 16 lanes a row
+    for (int e = tid >> 4; e < n * a.Hkv * 2; e += 16) {
+      const int kv = e & 1, g = e / 2 % a.Hkv, i = e / 2 / a.Hkv;
+      float f[8];
+      unpack8(((const uint4*)x)[path[i] * a.ldq + (long)(a.Hq + kv * a.Hkv + g) * 16 + c], f);
+      float am = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) am = fmaxf(am, fabsf(f[q]));
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) am = fmaxf(am, __shfl_xor(am, o, 16));
+      const float sc = am > 0.f ? am / 448.f : 1.f;
+      const uint2 w = f32x8_to_fp8(f, 1.f / sc);
+      const long slot = ((long)b * a.Hkv + g) * a.Smax + len + i;
+      char* const at = (char*)(kv ? a.vc : a.kc) + layer * a.layer + slot * 128;
+      *(uint2*)(at + (kv ? 8 * c : 32 * (c & 3) + 8 * (c >> 2))) = w;
+      if (c == 0) (kv ? a.vsc : a.ksc)[layer * a.sc_layer + ((long)b * a.Hkv + g) * a.SmaxP + len + i] = sc;
+    }
+    return;
+  }
   const long head = layer * a.layer + (long)b * a.Hkv * a.Smax * a.row;
   for (int e = tid; e < n * a.Hkv * a.row; e += 256) {
     const int i = e / (a.Hkv * a.row), r = e % (a.Hkv * a.row), g = r / a.row, c = r % a.row;
@@ -674,23 +760,23 @@ extern "C" int rt_draft_tree(const int* parent, const int* nodes, const int* pos
 
 constexpr int WIDE_ROWS = 192;  // rows of a key head that go to workgroups of 64
 
-template <int D, int RT, int WR, int WK, int KT>
+template <int D, int RT, int WR, int WK, int KT, bool KV8>
 static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
   TreeArgs t = a;
   t.blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
   const dim3 grid = t.blocks == 1 ? dim3(a.S, a.Hkv, a.B) : dim3(8 * t.blocks, (unsigned)(((long)a.S * a.B * a.Hkv + 7) / 8));
-  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT>), grid, dim3(64 * WR * WK), 0, stream, t);
+  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT, KV8>), grid, dim3(64 * WR * WK), 0, stream, t);
 }
-template <int D>
+template <int D, bool KV8>
 static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
   // waves by rows of 16, and two shares of each stage's keys: half the chain of a stage, and the shares are joined in LDS at the end (16 ungrouped
   // rows of 32 nodes 52 -> 47 us, 48 rows of 64 34 -> 31 against one share). Up to 192 rows go to workgroups of 64, two of them on a
   // CU, that read the same keys from L2 (32 rows of 128 over 500 to 2900 keys 56 us, in one workgroup of 8 waves with two tiles each 64); beyond, and
   // with few idle waves, two tiles a wave halve the reads of LDS (40 rows of 240 41 us against 46).
-  if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32>(a, rows, stream);
-  else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32>(a, rows, stream);
-  else if (rows <= WIDE_ROWS) launch_tree_form<D, 1, 4, 2, 32>(a, rows, stream);
-  else launch_tree_form<D, 2, 8, 1, 64>(a, rows, stream);
+  if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32, KV8>(a, rows, stream);
+  else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32, KV8>(a, rows, stream);
+  else if (rows <= WIDE_ROWS) launch_tree_form<D, 1, 4, 2, 32, KV8>(a, rows, stream);
+  else launch_tree_form<D, 2, 8, 1, 64, KV8>(a, rows, stream);
   RT_LAUNCH_CHECK();
   return 0;
 }
@@ -723,12 +809,13 @@ extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax, int
   return per + part * parts + join < 0.75f * stages ? parts : 1;
 }
 
-extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const int* kv_len, const int* kv_start,
-                                 const int64_t* see, void* o, long ldo, float* part, int S, int B, int N, int Hq, int Hkv, int D, int Smax,
+extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const float* ksc, const float* vsc, int SmaxP,
+                                 const int* kv_len, const int* kv_start, const int64_t* see, void* o, long ldo, float* part, int S, int B, int N, int Hq, int Hkv, int D, int Smax,
                                  int window, float scale, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
-  TreeArgs a{qkv, ldq, kc, vc, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, Hq / Hkv, 1.f / (Hq / Hkv), 0, 1, 0.f, 0.f, part, S};
+  TreeArgs a{qkv, ldq, kc, vc, ksc, vsc, SmaxP, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, Hq / Hkv, 1.f / (Hq / Hkv), 0, 1, 0.f, 0.f, part, S};
+  if (ksc && (!vsc || D != 128 || SmaxP < Smax || S < 1)) return -1;
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
     if (f32) hipLaunchKernelGGL(tree_any_kernel<float>, dim3(N, Hq, B), dim3(256), shm, stream, a);
@@ -743,7 +830,8 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   // Long rows first where a CU takes workgroups of 256 rows one after the other: 64 rows of 300 to 4000 keys in any order 177 us, as they come 230.
   // Smaller workgroups, of which several share a CU, only pay for the order (64 rows over 32 ungrouped heads 102 us, in order 110).
   a.sorted = rows > WIDE_ROWS && B > 1 && B <= 64 && (long)B * Hkv * S > num_cus();
-  const int rc = D == 128 ? launch_tree<128>(a, rows, stream) : launch_tree<64>(a, rows, stream);
+  const int rc = ksc ? launch_tree<128, true>(a, rows, stream) : D == 128 ? launch_tree<128, false>(a, rows, stream)
+                                                                          : launch_tree<64, false>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
     const long all = (long)B * Hkv * ((rows + 15) / 16) * (D / 16);
@@ -755,25 +843,30 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
 }
 
 extern "C" int rt_tree_accept(const int* parent, const int64_t* see, const int64_t* tokens, const int64_t* choice, const int* kv_len, int* count,
-                              int* path, int64_t* next, const void* const* drafts, long ldq, void* kc, void* vc, long layer, int B, int N, int L, int Hq,
+                              int* path, int64_t* next, const void* const* drafts, long ldq, void* kc, void* vc, long layer,
+                              float* ksc, float* vsc, long sc_layer, int SmaxP, int B, int N, int L, int Hq,
                               int Hkv, int Smax, int D, int size, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || L < 1 || L > LAYERS) return -1;
-  AcceptArgs a{parent, see, tokens, choice, kv_len, count, path, next, kc, vc, ldq, layer, B, N, L, Hq, Hkv, Smax, D, {}};
-  bool wide = (D * size) % 16 == 0 && (ldq * size) % 16 == 0 && (layer * size) % 16 == 0 && (uintptr_t)kc % 16 == 0 && (uintptr_t)vc % 16 == 0;
+  AcceptArgs a{parent, see, tokens, choice, kv_len, count, path, next, kc, vc, ldq, layer, ksc, vsc, sc_layer, SmaxP, B, N, L, Hq, Hkv, Smax, D, {}};
+  bool wide = (D * size) % 16 == 0 && (ldq * size) % 16 == 0 && layer * (ksc ? 1 : size) % 16 == 0 && (uintptr_t)kc % 16 == 0 && (uintptr_t)vc % 16 == 0;
   for (int i = 0; i < L; ++i) {
     a.drafts[i] = drafts[i];
     wide = wide && (uintptr_t)drafts[i] % 16 == 0;
   }
-  if (wide) {
+  if (ksc) {
+    if (!vsc || D != 128 || SmaxP < Smax || !wide) return -1;
+    a.ldq = ldq / 8;
+    hipLaunchKernelGGL((tree_accept_kernel<uint4, true>), dim3(B, L), dim3(256), 0, stream, a);
+  } else if (wide) {
     a.row = D * size / 16;
     a.ldq = ldq * size / 16;
     a.layer = layer * size / 16;
-    hipLaunchKernelGGL(tree_accept_kernel<uint4>, dim3(B, L), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((tree_accept_kernel<uint4, false>), dim3(B, L), dim3(256), 0, stream, a);
   } else if (size == 4) {
-    hipLaunchKernelGGL(tree_accept_kernel<uint32_t>, dim3(B, L), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((tree_accept_kernel<uint32_t, false>), dim3(B, L), dim3(256), 0, stream, a);
   } else {
-    hipLaunchKernelGGL(tree_accept_kernel<uint16_t>, dim3(B, L), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((tree_accept_kernel<uint16_t, false>), dim3(B, L), dim3(256), 0, stream, a);
   }
   RT_LAUNCH_CHECK();
   return 0;

@@ -477,10 +477,9 @@ class CausalLM(nn.Module):
     def verify(self, tokens, tree, kv_len, kv_start, cache):
         """One forward over drafted tokens [B, N] (``ops.draft_tree`` with pos0 = kv_len - kv_start): every node of a row is a row of its own that
         sees the row's cache and its ancestors. Returns (final hidden [B*N, H], the layers' rotated [q | k | v] rows, from which
-        ``ops.tree_accept`` appends the accepted nodes to the cache). bf16 / fp32 caches."""
+        ``ops.tree_accept`` appends the accepted nodes to the cache)."""
         cfg = self.cfg
-        if getattr(cache, "fp8", False):
-            raise ValueError("drafted tokens are checked over a bf16 or fp32 cache")
+        kv8 = getattr(cache, "fp8", False)
         cos, sin = self.rope(tokens.device)
         pos = tree.pos.reshape(-1)
         x = self.embed_tokens(tokens.reshape(-1), pos)
@@ -490,7 +489,8 @@ class CausalLM(nn.Module):
             if cos is not None and not rotated:
                 qkv = ops.rope_qkv(qkv, pos, cos, sin, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim)
             drafts.append(qkv)
-            o = ops.tree_attention(qkv, cache.k[li], cache.v[li], kv_len, tree, cfg.num_heads, kv_start, cfg.sliding_window)
+            ks, vs = cache.scales(li) if kv8 else (None, None)
+            o = ops.tree_attention(qkv, cache.k[li], cache.v[li], kv_len, tree, cfg.num_heads, kv_start, cfg.sliding_window, k_scale=ks, v_scale=vs)
             x, residual = layer.mlp(o, residual)
         return self.final_norm(x, residual), drafts
 

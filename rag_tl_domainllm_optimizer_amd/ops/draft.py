@@ -15,6 +15,7 @@ import torch
 
 from . import reference as ref
 from ._ext import native, on_gpu
+from .attention import FP8_KV_D, kv_dequantize, kv_quantize_rows
 
 MAX_NODES = 64  # a node's ancestors are the bits of one word
 
@@ -39,6 +40,17 @@ def _ints(t, name, shape, like):
     return t.contiguous()
 
 
+def _scales(k_cache, v_cache, k_scale, v_scale) -> bool:
+    """whether the caches are fp8, with the scales that go with them"""
+    fp8 = k_scale is not None
+    if fp8 != (v_scale is not None) or fp8 != (k_cache.dtype == torch.uint8) or v_cache.dtype != k_cache.dtype:
+        raise ValueError("an fp8 cache (uint8) has scales of its keys and values, another one has none")
+    if fp8 and (k_cache.shape[-1] != FP8_KV_D or any(s.dtype != torch.float32 or s.shape[:-1] != k_cache.shape[:-2] or s.shape[-1] < k_cache.shape[-2]
+                                                     for s in (k_scale, v_scale))):
+        raise ValueError(f"an fp8 cache has heads of {FP8_KV_D} and fp32 scales of every slot")
+    return fp8
+
+
 def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0: Optional[torch.Tensor] = None) -> DraftTree:
     """The plan of drafted trees: ``parent`` int32 [rows, nodes <= 64] holds an earlier node of the row for each (anything else: none, a tree of its
     own), ``nodes`` int32 [rows] how many of a row's are nodes (0: the row idles; default all), ``pos0`` int32 [rows] the position
@@ -55,13 +67,14 @@ def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0:
 
 def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, tree: DraftTree, Hq: int,
                    kv_start: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None,
-                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   out: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                   v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of drafted tokens -> [rows * nodes, Hq * D]. ``qkv`` [rows * nodes, >= (Hq + 2 Hkv) * D] holds the nodes' rotated rows [q | k | v];
     node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
     key; with ``window`` only those less than ``window`` positions before it. Nothing is appended to the caches; rows that are not
     nodes come out as zeros. ``out`` may be columns of wider rows, but shares nothing with ``qkv``. What other nodes hold, NaN among it, does not reach a node."""
     if on_gpu(qkv):
-        return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale)
+        return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     B, Hkv, Smax, D = k_cache.shape
@@ -70,8 +83,9 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"qkv: {B} rows of {N} nodes expected, got {tuple(qkv.shape)} for a tree {tuple(tree.shape)}")
     if Hkv < 1 or Hq < 1 or Hq % Hkv or qkv.shape[1] < (Hq + 2 * Hkv) * D:
         raise ValueError(f"{Hq} heads over {Hkv} of {D} do not fit {qkv.shape[1]} columns")
-    if k_cache.dtype != qkv.dtype or v_cache.dtype != qkv.dtype:
-        raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}: an fp8 cache is read by decode_step_attention only")
+    fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
+    if qkv.dtype != (torch.bfloat16 if fp8 else k_cache.dtype) and not (fp8 and qkv.dtype == torch.float32):
+        raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if window < 0 or not 0 < scale < math.inf:
         raise ValueError(f"window {window}, scale {scale}")
@@ -79,19 +93,22 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("tree_attention has no gradient")
     kv_len = _ints(kv_len, "kv_len", (B,), qkv)
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
+    if fp8:
+        k_cache, v_cache = (kv_dequantize(c, sc[..., :Smax], k) for c, sc, k in ((k_cache, k_scale, True), (v_cache, v_scale, False)))
     o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale)
     return o if out is None else out.copy_(o)
 
 
 def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, drafts: List[torch.Tensor], k_cache: torch.Tensor,
-                v_cache: torch.Tensor, kv_len: torch.Tensor):
+                v_cache: torch.Tensor, kv_len: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
     """The path that the model agrees with -> (its length int32 [rows], its nodes int32 [rows, nodes] (-1 behind them), the token after it int64
     [rows]). ``tokens`` / ``choice`` int64 [rows, nodes]: the drafted tokens, and what the model writes after each; the path starts at node 0 and goes
     on with the child whose token is the choice (the first of equal ones). Keys and values of its nodes go from ``drafts``
     (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
-    itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out."""
+    itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out.
+    ``k_scale`` / ``v_scale`` [layers, rows, Hkv, >= Smax]: the caches are fp8, and rows are rounded into them as ``kv_store_fp8`` does."""
     if on_gpu(k_cache):
-        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len)
+        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale)
     if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     L, B, Hkv, Smax, D = k_cache.shape
@@ -101,8 +118,10 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
         raise ValueError("tokens and choice: int64 expected")
     if D < 1 or Hkv < 1:
         raise ValueError("caches of no heads")
-    if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or x.dtype != k_cache.dtype or x.shape[0] != B * tree.shape[1]
+    fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
+    if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or (x.dtype != k_cache.dtype and not fp8) or x.shape[0] != B * tree.shape[1]
                                or x.shape[1] % D or x.shape[1] <= 2 * Hkv * D for x in drafts):
         raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")
     kv_len = _ints(kv_len, "kv_len", (B,), k_cache)
-    return ref.tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len)
+    store = (lambda x, k: kv_quantize_rows(x, k)) if fp8 else None
+    return ref.tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, store, k_scale, v_scale)

@@ -438,7 +438,7 @@ def tree_attention(qkv, kc, vc, kv_len, see, Hq, kv_start=None, window=0, scale=
     return out.view(B * N, Hq * D).to(qkv.dtype)
 
 
-def tree_accept(parent, see, tokens, choice, drafts, kc, vc, kv_len):
+def tree_accept(parent, see, tokens, choice, drafts, kc, vc, kv_len, store=None, ksc=None, vsc=None):
     L, B, Hkv, Smax, D = kc.shape
     N = see.shape[1]
     count = torch.zeros(B, dtype=torch.int32, device=kc.device)
@@ -458,8 +458,10 @@ def tree_accept(parent, see, tokens, choice, drafts, kc, vc, kv_len):
         nodes = nodes[:max(Smax - at, 0)]
         for layer, x in enumerate(drafts):
             rows = x.view(B, N, -1, D)[b, nodes].transpose(0, 1)
-            kc[layer, b, :, at:at + len(nodes)] = rows[-2 * Hkv:-Hkv]
-            vc[layer, b, :, at:at + len(nodes)] = rows[-Hkv:]
+            for c, sc, new, k in ((kc, ksc, rows[-2 * Hkv:-Hkv], True), (vc, vsc, rows[-Hkv:], False)):
+                if store is not None:
+                    new, sc[layer, b, :, at:at + len(nodes)] = store(new, k)
+                c[layer, b, :, at:at + len(nodes)] = new
     return count, path, after
 
 

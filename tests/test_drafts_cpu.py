@@ -217,11 +217,69 @@ def _depth(up, i):
     return 0 if up[i] < 0 else 1 + _depth(up, up[i])
 
 
-def test_an_fp8_cache_is_refused():
-    cfg = models.resolve_preset("tiny-mistral")
-    m = models.CausalLM(cfg, dtype=torch.float32)
+def _fp8(*shape, seed=0):
+    """an fp8 cache [.., slots, 128] of random rows, its scales with three slots more, and what it holds"""
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+    return x, [ops.kv_quantize_rows(x, k) for k in (True, False)]
 
-    class Cache:
-        fp8 = True
+
+def test_attention_over_an_fp8_cache():
+    B, N, Hq, Hkv, D = 2, 5, 4, 2, 128
+    _, ((kq, ks), (vq, vs)) = _fp8(B, Hkv, 20, D)
+    kd, vd = ops.kv_dequantize(kq, ks, True), ops.kv_dequantize(vq, vs, False)
+    qkv, parents = torch.randn(B * N, (Hq + 2 * Hkv) * D), plain.trees(B, N, 0)
+    pad = lambda t: torch.nn.functional.pad(t, (0, 3), value=math.nan)
+    o = ops.tree_attention(qkv, kq, vq, torch.tensor([20, 7], dtype=torch.int32), _tree(parents), Hq, k_scale=pad(ks), v_scale=pad(vs))
+    want, size = plain.attention(qkv, kd, vd, [20, 7], parents, [N, N], Hq)
+    assert ((o - want).abs() <= 2 ** -24 * (16 * D + 64) * size).all()  # fp32: 128 products and sums of a score below 16, and as many of the keys
+
+
+def test_accept_into_an_fp8_cache():
+    B, N, L, Hq, Hkv, D, slots = 2, 4, 2, 2, 2, 128, 9
+    x = [torch.randn(B * N, (Hq + 2 * Hkv) * D) for _ in range(L)]
+    kc, vc = torch.zeros(L, B, Hkv, slots, D, dtype=torch.uint8), torch.zeros(L, B, Hkv, slots, D, dtype=torch.uint8)
+    ks, vs = torch.zeros(L, B, Hkv, 16), torch.zeros(L, B, Hkv, 16)
+    tokens = torch.arange(N).repeat(B, 1)
+    count, path, after = ops.tree_accept(_tree([[-1, 0, 1, 2]] * B, [4, 1]), tokens, (tokens + 1) % 4, x, kc, vc, torch.tensor([5, 7], dtype=torch.int32), ks, vs)
+    assert count.tolist() == [4, 1] and after.tolist() == [0, 1]
+    for b, n, at in ((0, 4, 5), (1, 1, 7)):
+        for layer in range(L):
+            rows = x[layer].view(B, N, -1, D)[b, :n].transpose(0, 1)
+            for c, sc, new, k in ((kc, ks, rows[Hq:Hq + Hkv], True), (vc, vs, rows[Hq + Hkv:], False)):
+                q, s = ops.kv_quantize_rows(new, k)
+                assert torch.equal(c[layer, b, :, at:at + n], q) and torch.equal(sc[layer, b, :, at:at + n], s)
+                assert (c[layer, b, :, :at] == 0).all() and (sc[layer, b, :, :at] == 0).all() and (c[layer, b, :, at + n:] == 0).all()
+
+
+@pytest.mark.parametrize("bad", [
+    lambda k, v, ks, vs, t, n: ops.tree_attention(torch.zeros(2, 512), k, v, n, t, 2),
+    lambda k, v, ks, vs, t, n: ops.tree_attention(torch.zeros(2, 512), k, v, n, t, 2, k_scale=ks),
+    lambda k, v, ks, vs, t, n: ops.tree_attention(torch.zeros(2, 512), k, v, n, t, 2, k_scale=ks[..., :3], v_scale=vs[..., :3]),
+    lambda k, v, ks, vs, t, n: ops.tree_attention(torch.zeros(2, 512), k.float(), v.float(), n, t, 2, k_scale=ks, v_scale=vs),
+    lambda k, v, ks, vs, t, n: ops.tree_attention(torch.zeros(2, 256), k[..., :64], v[..., :64], n, t, 2, k_scale=ks, v_scale=vs),
+    lambda k, v, ks, vs, t, n: ops.tree_accept(t, torch.zeros(1, 2, dtype=torch.int64), torch.zeros(1, 2, dtype=torch.int64), [torch.zeros(2, 512)], k[None], v[None], n),
+])
+def test_fp8_caches_without_their_scales_are_refused(bad):
+    _, ((k, ks), (v, vs)) = _fp8(1, 1, 9, 128)
     with pytest.raises(ValueError):
-        m.verify(torch.zeros(1, 1, dtype=torch.long), _tree([[-1]]), torch.zeros(1, dtype=torch.int32), None, Cache())
+        bad(k, v, ks, vs, _tree([[-1, 0]]), torch.zeros(1, dtype=torch.int32))
+
+
+def test_answers_written_by_drafts_over_an_fp8_cache():
+    """the model passes the scales on: the prompt and the accepted path lie quantised in the cache, and each step's states are those of attending over it"""
+    cfg = models.ModelConfig(arch="mistral", vocab_size=64, hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, head_dim=128, intermediate_size=256,
+                             max_position=64, norm_eps=1e-5, name="two-heads")
+    m = models.CausalLM(cfg, dtype=torch.float32, seed=1)
+    q, b = (KVCache(2, 1, 1, 32, 128, "cpu", torch.float32, fp8=fp8) for fp8 in (True, False))
+    m.prefill(torch.tensor([[3, 9, 27, 17]]), torch.zeros(1, dtype=torch.int32), q)
+    kv_len = torch.tensor([4], dtype=torch.int32)
+    for step in range(2):
+        for layer in range(2):
+            b.k[layer].copy_(ops.kv_dequantize(q.k[layer], q.ks[layer][..., :32], True))
+            b.v[layer].copy_(ops.kv_dequantize(q.v[layer], q.vs[layer][..., :32], False))
+        tree, tokens = ops.draft_tree(torch.tensor([[-1, 0, 0, 1]], dtype=torch.int32), pos0=kv_len), torch.tensor([[5, 6, 7, 8]])
+        h, drafts = m.verify(tokens, tree, kv_len, None, q)
+        assert torch.allclose(h, m.verify(tokens, tree, kv_len, None, b)[0], rtol=1e-5, atol=1e-6)
+        count, path, after = ops.tree_accept(tree, tokens, torch.tensor([[6, 8, 0, 1]]), drafts, q.k, q.v, kv_len, q.ks, q.vs)
+        assert path.tolist() == [[0, 1, 3, -1]] and after.tolist() == [1]
+        kv_len = kv_len + count

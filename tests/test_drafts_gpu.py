@@ -42,7 +42,7 @@ def test_plan_of_odd_parents():
 
 
 # ------------------------------------------------------------------------------------------ attention
-def _attention(Hq, Hkv, D, N, lens, slots, starts=None, counts=None, window=0, dtype=BF16, seed=0, extra=0, junk=math.nan):
+def _attention(Hq, Hkv, D, N, lens, slots, starts=None, counts=None, window=0, dtype=BF16, seed=0, extra=0, junk=math.nan, fp8=False):
     B = len(lens)
     counts = counts or [N] * B
     parents = plain.trees(B, N, seed)
@@ -56,7 +56,17 @@ def _attention(Hq, Hkv, D, N, lens, slots, starts=None, counts=None, window=0, d
         qkv[b * N + counts[b]:(b + 1) * N] = junk
     out = torch.full((B * N, Hq * D), 7.0, dtype=dtype, device=DEV)
     tree = ops.draft_tree(_i32(parents), _i32(counts))
-    ops.tree_attention(qkv, kc, vc, _i32(lens), tree, Hq, _i32(starts), window, out=out)
+    held, scales = (kc, vc), {}
+    if fp8:
+        (kq, ks), (vq, vs) = (ops.kv_quantize_rows(c.nan_to_num(), k) for c, k in ((kc, True), (vc, False)))
+        kc, vc = ops.kv_dequantize(kq, ks, True), ops.kv_dequantize(vq, vs, False)
+        for b in range(B):
+            for c, sc in ((kq, ks), (vq, vs)):  # no numbers where nothing is seen
+                c[b, :, lens[b]:], sc[b, :, lens[b]:] = 0x7f, math.nan
+                if starts:
+                    c[b, :, :starts[b]], sc[b, :, :starts[b]] = 0x7f, math.nan
+        held, scales = (kq, vq), dict(k_scale=torch.nn.functional.pad(ks, (0, 5)), v_scale=torch.nn.functional.pad(vs, (0, 5)))
+    ops.tree_attention(qkv, *held, _i32(lens), tree, Hq, _i32(starts), window, out=out, **scales)
     want, size = plain.attention(torch.nan_to_num(qkv), kc, vc, lens, parents, counts, Hq, starts, window)
     # the output's rounding, half a step of its value; p rounded to the cache's type in front of the product with v, half a step
     # of each term; fp32 scores: D products and sums of 2^-24 each of sum |q k| scale (below 16 here), which p takes over as a
@@ -124,6 +134,43 @@ def test_attention_long(lens, N):
 @pytest.mark.parametrize("Hq,Hkv,D,N", [(8, 2, 128, 7), (4, 4, 64, 33), (3, 1, 20, 4)])
 def test_attention_f32(Hq, Hkv, D, N):
     _attention(Hq, Hkv, D, N, [100, 0, 31], 120, dtype=F32, window=50, junk=2.0)
+
+
+@pytest.mark.parametrize("Hq,Hkv,N", [(4, 4, 1), (5, 5, 16), (8, 2, 8), (32, 8, 16), (8, 2, 33), (8, 2, 64), (12, 1, 64)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_over_an_fp8_cache(Hq, Hkv, N, window):
+    _attention(Hq, Hkv, 128, N, [130, 0, 1, 64, 65, 191], 200, starts=[0, 0, 0, 10, 64, 3], counts=[N, N, N, 1, N, 0], window=window, seed=N, fp8=True)
+
+
+@pytest.mark.parametrize("lens", [[2100], [900, 9, 700]])
+@pytest.mark.parametrize("N", [2, 30, 60])
+def test_attention_over_a_long_fp8_cache(lens, N):
+    _attention(8, 2, 128, N, lens, max(lens) + 5, fp8=True, extra=3 if N == 2 else 0)
+
+
+@pytest.mark.parametrize("extra", [0, 3])
+@pytest.mark.parametrize("N", [1, 7, 64])
+def test_accept_into_an_fp8_cache(N, extra):
+    r = random.Random(N)
+    B, L, Hq, Hkv, D, slots = 5, 3, 4, 2, 128, 80
+    parents, counts = plain.trees(B, N, N, 3), [N] + [r.randint(0, N) for _ in range(B - 1)]
+    parents[0] = [-1] + list(range(N - 1))
+    tokens, choice = ([[r.randrange(3) for _ in range(N)] for _ in range(B)] for _ in "tc")
+    choice[0] = tokens[0][1:] + [9]
+    lens = [20] + [r.randint(0, slots) for _ in range(B - 1)]
+    rows = [_rand(B * N, (Hq + 2 * Hkv) * D + extra, seed=i) for i in range(L)]
+    rows[0][0, Hq * D:(Hq + 1) * D] = 0  # a key of zeros
+    drafts = [x[:, :(Hq + 2 * Hkv) * D] for x in rows]
+    t = lambda x: torch.tensor(x)
+    out = []
+    for dev in ("cpu", DEV):
+        kc, vc = (torch.full((L, B + 1, Hkv, slots, D), 3, dtype=torch.uint8, device=dev) for _ in "kv")
+        ks, vs = (torch.full((L, B + 1, Hkv, 96), 2.0, device=dev) for _ in "kv")
+        tree = ops.draft_tree(t(parents).int().to(dev), t(counts).int().to(dev))
+        o = ops.tree_accept(tree, t(tokens).to(dev), t(choice).to(dev), drafts if dev == DEV else [x.cpu() for x in drafts], kc[:, :B], vc[:, :B], t(lens).int().to(dev), ks[:, :B], vs[:, :B])
+        out.append([x.cpu() for x in (*o, kc, vc, ks, vs)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b)
 
 
 def test_attention_of_rows_with_an_odd_pitch():
@@ -546,6 +593,12 @@ def test_runs_repeat_bit_by_bit():
     lambda: ops.tree_attention(_rand(2, 512), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4,
                                out=torch.empty(1, 256, dtype=BF16, device=DEV).expand(2, 256)),
     lambda: _in_place(_rand(2, 512)),
+    lambda: ops.tree_attention(_rand(2, 512, dtype=F32), *(torch.zeros(1, 1, 9, 128, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]),
+                               ops.draft_tree(_i32([[-1, 0]])), 2, k_scale=torch.ones(1, 1, 9, device=DEV), v_scale=torch.ones(1, 1, 9, device=DEV)),
+    lambda: ops.tree_attention(_rand(2, 512), *(torch.zeros(1, 1, 9, 128, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]),
+                               ops.draft_tree(_i32([[-1, 0]])), 2, k_scale=torch.ones(1, 1, 8, device=DEV), v_scale=torch.ones(1, 1, 8, device=DEV)),
+    lambda: ops.tree_attention(_rand(2, 512), *(_rand(1, 1, 9, 128) for _ in "kv"), _i32([3]),
+                               ops.draft_tree(_i32([[-1, 0]])), 2, k_scale=torch.ones(1, 1, 9, device=DEV), v_scale=torch.ones(1, 1, 9, device=DEV)),
     lambda: ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.long, device=DEV) for _ in "tc"), [_rand(2, 512)],
                             *(torch.zeros(1, 1, 2, 9, 0, dtype=BF16, device=DEV) for _ in "kv"), _i32([3])),
     lambda: ops.token_alternatives(_rand(2, 50), None, 33),
