@@ -197,12 +197,14 @@ __device__ __forceinline__ int longest(const TreeArgs& a, int q, int lane) {
 // one v_maximum3_f32 for two of these; fmaxf has each operand made canonical first. A NaN stays one.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// The bound: 128 registers, for two workgroups of eight waves in a CU, where the e4m3 form alone would take 162 (rows of 128 queries: 81
+// instead of 91 us; with a window, whose first stages then read some of them back from scratch, 17.7 instead of 15.6).
 template <int D, int RT, int WR, int WK, int KT, bool KV8>
-__global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
   static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
-  __shared__ __attribute__((aligned(16))) float scales[KV8 ? 2 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
+  __shared__ __attribute__((aligned(16))) float scales[KV8 ? 4 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
   __shared__ unsigned bad[2];  // keys of the nodes' stage whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   // (part, key head, row); where several workgroups share a key head's rows, the grid is (8 x these, all of the former by eight): blocks go to
@@ -303,49 +305,55 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         }
       }
     };
-    // a stage of an e4m3 cache: to registers while the stage before is multiplied, then as bf16 (exact) to LDS
-    constexpr int NU = KV8 ? SK * D / 16 / (64 * NW) : 1;
-    uint4 rk[NU], rv[NU];
-    float rs = 0.f;
+    // An e4m3 cache: two stages are on their way to LDS as they are, in the second half of the buffers; a stage is made bf16 (exact) in the
+    // first half when its turn comes. The nodes' stage, in bf16, takes the second half once the last of these has left it. Measured against
+    // the next stage's bytes in registers, and against a cache in bf16: 64 rows of 48 nodes over 100 to 700 keys in 32 key heads of one
+    // query each 117 -> 77 us (bf16 93), 48 rows of 16 nodes over 150 to 1200 keys in 8 heads of four 45 -> 39 (29), 64 rows of 64 nodes over
+    // 200 to 4000 keys 246 -> 231 (213): half the bytes, but a pass over LDS and a barrier for them, so it wins where memory bounds the bf16 form.
+    const int raw_end = min(t1, ct.tiles - 1);
     auto fetch = [&](int tile) {
+      const int last = ct.len - ct.lo - tile * SK - 1, slot = tile - t0;
       const long at = head + ((long)ct.lo + (long)tile * SK) * D;
-      const int last = ct.len - ct.lo - tile * SK - 1;
+      char* const dst = smem + 2 * KB + (slot & 1) * KB + wid * 1024;
 #pragma unroll
-      for (int j = 0; j < NU; ++j) {
-        const int e = j * 64 * NW + tid;
-        const long from = at + min(e / 8, last) * D + e % 8 * 16;
-        rk[j] = *(const uint4*)((const char*)a.kc + from);
-        rv[j] = *(const uint4*)((const char*)a.vc + from);
+      for (int j = 0; j < NJ / 2; ++j) {
+        const int e = (j * NW + wid) * 64 + lane;
+        const uint32_t from = min(e / 8, last) * D + e % 8 * 16;
+        paged::lds_dma16((const char*)a.kc + at, from, dst + j * NW * 1024);
+        paged::lds_dma16((const char*)a.vc + at, from, dst + KB / 2 + j * NW * 1024);
       }
-      if (tid < 2 * SK) rs = (tid < SK ? a.ksc : a.vsc)[pair_at * a.SmaxP + ct.lo + tile * SK + min(tid % SK, last)];
+      const long sc = pair_at * a.SmaxP + ct.lo + tile * SK;
+      paged::lds_dma4(a.ksc + sc, 4 * min(lane, last), scales[slot & 3]);  // by every wave: the same to the same place
+      paged::lds_dma4(a.vsc + sc, 4 * min(lane, last), scales[slot & 3] + SK);
     };
-    auto settle = [&](int buf) {
-      char* const img = smem + 2 * buf * KB;
+    constexpr int RAW_LOADS = NJ / 2 * 2 + 2;
+    auto convert = [&](int tile) {
+      const char* const raw = smem + 2 * KB + (tile - t0 & 1) * KB;
 #pragma unroll
-      for (int j = 0; j < NU; ++j) {
+      for (int j = 0; j < SK * D / 16 / (64 * NW); ++j) {
         // 16 bytes h of a key: elements 8 (4 s + h / 2) .. + 7 of s = 2 (h % 2) and the next; of a value 16 h .. 16 h + 15
         const int e = j * 64 * NW + tid, key = e / 8, h = e % 8, c = 8 * (h % 2) + h / 2;
-        *(bf16x8*)(img + paged::kq_off<D>(key, c)) = fp8x8_to_bf16(rk[j].x, rk[j].y);
-        *(bf16x8*)(img + paged::kq_off<D>(key, c + 4)) = fp8x8_to_bf16(rk[j].z, rk[j].w);
-        *(bf16x8*)(img + KB + paged::vv_off<D>(key, 2 * h)) = fp8x8_to_bf16(rv[j].x, rv[j].y);
-        *(bf16x8*)(img + KB + paged::vv_off<D>(key, 2 * h + 1)) = fp8x8_to_bf16(rv[j].z, rv[j].w);
+        const uint4 k = *(const uint4*)(raw + 16 * e), v = *(const uint4*)(raw + KB / 2 + 16 * e);
+        *(bf16x8*)(smem + paged::kq_off<D>(key, c)) = fp8x8_to_bf16(k.x, k.y);
+        *(bf16x8*)(smem + paged::kq_off<D>(key, c + 4)) = fp8x8_to_bf16(k.z, k.w);
+        *(bf16x8*)(smem + KB + paged::vv_off<D>(key, 2 * h)) = fp8x8_to_bf16(v.x, v.y);
+        *(bf16x8*)(smem + KB + paged::vv_off<D>(key, 2 * h + 1)) = fp8x8_to_bf16(v.z, v.w);
       }
-      if (tid < 2 * SK) scales[buf][tid] = rs;
     };
     if (tid < 2) bad[tid] = 0;
-    if (KV8 && t0 < ct.tiles - 1) {
+    if (KV8 && t0 < raw_end) {
       fetch(t0);
-      settle(0);
+      if (t0 + 1 < raw_end) fetch(t0 + 1);
     } else {
-      stage(t0, 0);
+      stage(t0, KV8);
     }
-    int cur = 0;
+    int cur = KV8;
     // a stage that lies in LDS; MODE 0: every row sees all of its keys, 1: some keys of the context are not seen, 2: the nodes' own keys
-    auto multiply = [&](auto mode, int t, int now) {
+    auto multiply = [&](auto mode, int t, char* image) {
       constexpr int MODE = decltype(mode)::value;
       constexpr bool SCALED = KV8 && MODE != 2;
-      char* const Ks = smem + 2 * now * KB + wk * KT * D * 2;
-      char* const Vs = smem + (2 * now + 1) * KB + wk * KT * D * 2;
+      char* const Ks = image + wk * KT * D * 2;
+      char* const Vs = Ks + KB;
       f32x4 st[KS][RT];
 #pragma unroll
       for (int k = 0; k < KS; ++k)
@@ -364,7 +372,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
       if constexpr (SCALED) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const f32x4 sc = *(const f32x4*)&scales[now][key0 + 16 * k];
+          const f32x4 sc = *(const f32x4*)&scales[t - t0 & 3][key0 + 16 * k];
 #pragma unroll
           for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -438,7 +446,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
       if constexpr (SCALED) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const f32x4 sc = *(const f32x4*)&scales[now][SK + key0 + 16 * k];
+          const f32x4 sc = *(const f32x4*)&scales[t - t0 & 3][SK + key0 + 16 * k];
 #pragma unroll
           for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -499,17 +507,27 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
     };
     auto turn = [&](auto mode, int t) {
       constexpr int MODE = decltype(mode)::value;
+      if constexpr (KV8 && MODE != 2) {
+        if (t + 1 < raw_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(RAW_LOADS) : "memory");  // this stage, not the next one
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");  // ... of every wave, and the stage before is multiplied
+        convert(t);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+        if (t + 2 < raw_end) fetch(t + 2);
+        else if (t + 2 == ct.tiles && t + 1 < t1) stage(t + 1, 1);
+        if (row0 < M) multiply(mode, t, smem);
+        return;
+      }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
       asm volatile("s_barrier" ::: "memory");                      // ... by every wave; the other buffer is free
-      const bool more = MODE != 2 && t + 1 < t1, more8 = KV8 && more && t + 1 < ct.tiles - 1;
-      if (more8) fetch(t + 1);
-      else if (more) stage(t + 1, cur ^ 1);
-      const int now = cur;
+      if (MODE != 2 && t + 1 < t1) stage(t + 1, cur ^ 1);
+      char* const image = smem + 2 * cur * KB;
       cur ^= 1;
       if constexpr (MODE == 2) {
         // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
         // product and are added below for the rows that see them
-        char* const img = smem + (2 * now + 1) * KB;
+        char* const img = image + KB;
         for (int e = tid; e < NODES * NC; e += 64 * NW) {
           uint32_t* const w = (uint32_t*)(img + e * 16);
 #pragma unroll
@@ -523,8 +541,7 @@ __global__ __launch_bounds__(64 * WR * WK) void tree_mfma_kernel(TreeArgs a) {
         }
         __syncthreads();
       }
-      if (row0 < M) multiply(mode, t, now);
-      if (more8) settle(cur);
+      if (row0 < M) multiply(mode, t, image);
     };
     int t = t0;
     if (a.window)  // stages that the last nodes do not see all of
