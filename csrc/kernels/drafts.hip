@@ -197,15 +197,28 @@ __device__ __forceinline__ int longest(const TreeArgs& a, int q, int lane) {
 // one v_maximum3_f32 for two of these; fmaxf has each operand made canonical first. A NaN stays one.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// The bound: 128 registers, for two workgroups of eight waves in a CU, where the e4m3 form alone would take 162 (rows of 128 queries: 81
-// instead of 91 us; with a window, whose first stages then read some of them back from scratch, 17.7 instead of 15.6).
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 B at an address of LDS and 16 B `second` behind it. An ordinary read would wait for every DMA to LDS that is under way.
+template <int second>
+__device__ __forceinline__ void read_pair(uint32_t at, u32x4& x, u32x4& y) {
+  asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x), "=&v"(y) : "v"(at), "i"(second) : "memory");
+}
+
+// e4m3 byte e of four
+__device__ __forceinline__ float fp8_at(uint32_t four, int e) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+  const f32x2_t f = e < 2 ? __builtin_amdgcn_cvt_pk_f32_fp8(four, false) : __builtin_amdgcn_cvt_pk_f32_fp8(four, true);
+  return f[e & 1];
+}
+
+// The bound: 128 registers, for two workgroups of eight waves in a CU (e4m3, rows of 128 queries, when it took 162: 91 us, and 81 with the bound).
 template <int D, int RT, int WR, int WK, int KT, bool KV8>
-__global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfma_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
   static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
   __shared__ __attribute__((aligned(16))) char smem[4 * KB];
   __shared__ __attribute__((aligned(16))) float scales[KV8 ? 4 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
-  __shared__ unsigned bad[2];  // keys of the nodes' stage whose values are not all numbers
+  __shared__ unsigned bad[2][2];  // keys of the first stage, and of the nodes', whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   // (part, key head, row); where several workgroups share a key head's rows, the grid is (8 x these, all of the former by eight): blocks go to
   // the eight XCDs in turn, and those that read the same keys come eight later, to the same L2
@@ -309,7 +322,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
     // first half when its turn comes. The nodes' stage, in bf16, takes the second half once the last of these has left it. Measured against
     // the next stage's bytes in registers, and against a cache in bf16: 64 rows of 48 nodes over 100 to 700 keys in 32 key heads of one
     // query each 117 -> 77 us (bf16 93), 48 rows of 16 nodes over 150 to 1200 keys in 8 heads of four 45 -> 39 (29), 64 rows of 64 nodes over
-    // 200 to 4000 keys 246 -> 231 (213): half the bytes, but a pass over LDS and a barrier for them, so it wins where memory bounds the bf16 form.
+    // 1000 to 4000 keys 246 -> 231 (213): half the bytes, but a pass over LDS and a barrier for them, so it wins where memory bounds the bf16 form.
     const int raw_end = min(t1, ct.tiles - 1);
     auto fetch = [&](int tile) {
       const int last = ct.len - ct.lo - tile * SK - 1, slot = tile - t0;
@@ -340,7 +353,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
         *(bf16x8*)(smem + KB + paged::vv_off<D>(key, 2 * h + 1)) = fp8x8_to_bf16(v.z, v.w);
       }
     };
-    if (tid < 2) bad[tid] = 0;
+    if (tid < 4) bad[tid / 2][tid & 1] = 0;
     if (KV8 && t0 < raw_end) {
       fetch(t0);
       if (t0 + 1 < raw_end) fetch(t0 + 1);
@@ -348,7 +361,8 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
       stage(t0, KV8);
     }
     int cur = KV8;
-    // a stage that lies in LDS; MODE 0: every row sees all of its keys, 1: some keys of the context are not seen, 2: the nodes' own keys
+    // a stage that lies in LDS; MODE 0: every row sees all of its keys, 1: a window leaves out keys of the context for some, 2: the nodes'
+    // own keys, 3: the context's last keys, repeated behind its end
     auto multiply = [&](auto mode, int t, char* image) {
       constexpr int MODE = decltype(mode)::value;
       constexpr bool SCALED = KV8 && MODE != 2;
@@ -390,7 +404,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
               if (!(bits >> e & 1)) st[k][u][e] = -INFINITY;
           }
       }
-      if constexpr (MODE == 1) {
+      if constexpr (MODE == 1 || MODE == 3) {
         const int first = ct.lo + t * SK + key0;
 #pragma unroll
         for (int u = 0; u < RT; ++u)
@@ -399,7 +413,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int key = first + 16 * k + e;
-              if (key >= ct.len || key < from[u]) st[k][u][e] = -INFINITY;
+              if (key >= ct.len || (MODE == 1 && key < from[u])) st[k][u][e] = -INFINITY;
             }
       }
       bool grown = false;
@@ -450,7 +464,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
 #pragma unroll
           for (int u = 0; u < RT; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[k][u][e] *= sc[e];
+            for (int e = 0; e < 4; ++e) st[k][u][e] *= MODE == 0 || (MODE == 1 ? fabsf(sc[e]) < INFINITY : key0 + 16 * k + e < ct.rest) ? sc[e] : 0.f;
         }
       }
       bf16x8 pf[KT / 32][RT];
@@ -458,6 +472,25 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
       for (int k = 0; k < KT / 32; ++k)
 #pragma unroll
         for (int u = 0; u < RT; ++u) pf[k][u] = paged::pack_p(st[2 * k][u], st[2 * k + 1][u]);
+      // 0 times the infinity that the last key's value may be is no number: its repetitions count as 0
+      uint32_t real[KT / 32][4];
+      if constexpr (MODE == 3)
+#pragma unroll
+        for (int k = 0; k < KT / 32; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int left = ct.rest - (key0 + 32 * k + 16 * (i / 2) + 2 * (i & 1));
+            real[k][i] = left <= 0 ? 0 : left == 1 ? 0xffffu : ~0u;
+          }
+      auto of_keys = [&](bf16x8 v, int k) {
+        if constexpr (MODE == 3) {
+          u32x4 w = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] &= real[k][i];
+          v = __builtin_bit_cast(bf16x8, w);
+        }
+        return v;
+      };
       const int key_a = 4 * g + (lane >> 2 & 3), pcol = lane & 3;  // transposed reads: rows 16 apart have the same swizzle
 #pragma unroll
       for (int c = 0; c < DT; c += 4) {
@@ -471,7 +504,7 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const bf16x8 vf = paged::cat4(v[4 * k + 2 * h], v[4 * k + 2 * h + 1]);
+              const bf16x8 vf = of_keys(paged::cat4(v[4 * k + 2 * h], v[4 * k + 2 * h + 1]), h);
 #pragma unroll
               for (int u = 0; u < RT; ++u) o[u][c + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[h][u], o[u][c + k], 0, 0, 0);
             }
@@ -481,27 +514,32 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
           ds_tr16_at8(at, v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const bf16x8 vf = paged::cat4(v[2 * k], v[2 * k + 1]);
+            const bf16x8 vf = of_keys(paged::cat4(v[2 * k], v[2 * k + 1]), 0);
 #pragma unroll
             for (int u = 0; u < RT; ++u) o[u][c + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[0][u], o[u][c + k], 0, 0, 0);
           }
         }
       }
-      if constexpr (MODE == 2) {
-        const uint64_t ill = ((uint64_t)bad[1] << 32 | bad[0]) & (KT == 64 ? ~0ull : 0xffffffffull << (wk * KT));
-        for (uint64_t w = ill; w; w &= w - 1) {
-          const int key = __builtin_ctzll(w);
-          const bf16_t* const v = (key < joint ? vc + ((long)ct.full * SK + key) * D : nv + (long)(key - joint) * a.ldq) + 4 * g;
+    };
+    // The values of a stage that some row does not see all of: 0 times what is no number is none, so such values count as 0 in the product and
+    // are added at the end for the rows that see them. These are the nodes' stage and, with a window, the first one (the last node's starts less
+    // than NODES keys behind the first one's). The reads are of this kind because ordinary ones would wait for the next stage.
+    auto only_numbers = [&](char* values, bool own) {
+      constexpr int second = KB / 2;
+#pragma unroll 1
+      for (int e = 16 * tid; e < second; e += 16 * 64 * NW) {
+        u32x4 w[2];
+        read_pair<second>(lds_addr(values + e), w[0], w[1]);
 #pragma unroll
-          for (int u = 0; u < RT; ++u)
-            if (sees[u] >> key & 1)
+        for (int h = 0; h < 2; ++h) {
+          const int key = (e + h * second) / (2 * D);
+          u32x4 x = w[h];
 #pragma unroll
-              for (int c = 0; c < DT; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float f = bf2f(v[16 * c + e]);
-                  if (!(fabsf(f) < INFINITY)) o[u][c][e] += f;
-                }
+          for (int i = 0; i < 4; ++i) x[i] &= ((x[i] & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((x[i] & 0x7f800000u) == 0x7f800000u ? 0xffffu : ~0u);
+          bool ill = x[0] != w[h][0] || x[1] != w[h][1] || x[2] != w[h][2] || x[3] != w[h][3];
+          if (ill) *(u32x4*)(values + e + h * second) = x;
+          if (KV8 && !own) ill |= !(fabsf(scales[0][SK + key]) < INFINITY);
+          if (ill) atomicOr(&bad[own][key / 32], 1u << (key % 32));
         }
       }
     };
@@ -514,6 +552,11 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
         convert(t);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
+        if constexpr (MODE == 1) {
+          only_numbers(smem + KB, false);
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          asm volatile("s_barrier" ::: "memory");
+        }
         if (t + 2 < raw_end) fetch(t + 2);
         else if (t + 2 == ct.tiles && t + 1 < t1) stage(t + 1, 1);
         if (row0 < M) multiply(mode, t, smem);
@@ -524,31 +567,42 @@ __global__ __launch_bounds__(64 * WR * WK, KV8 && WR == 4 ? 4 : 1) void tree_mfm
       if (MODE != 2 && t + 1 < t1) stage(t + 1, cur ^ 1);
       char* const image = smem + 2 * cur * KB;
       cur ^= 1;
-      if constexpr (MODE == 2) {
-        // a node's values must not reach the nodes beside it, and 0 times what is no number is none: such values count as 0 in the
-        // product and are added below for the rows that see them
-        char* const img = image + KB;
-        for (int e = tid; e < NODES * NC; e += 64 * NW) {
-          uint32_t* const w = (uint32_t*)(img + e * 16);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const bool lo = (w[i] & 0x7f80u) == 0x7f80u, hi = (w[i] & 0x7f800000u) == 0x7f800000u;
-            if (lo || hi) {
-              w[i] &= (lo ? 0xffff0000u : ~0u) & (hi ? 0xffffu : ~0u);
-              atomicOr(&bad[e / NC / 32], 1u << (e / NC % 32));
-            }
-          }
-        }
-        __syncthreads();
+      if constexpr (MODE == 1 || MODE == 2) {
+        only_numbers(image + KB, MODE == 2);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
       }
       if (row0 < M) multiply(mode, t, image);
     };
     int t = t0;
-    if (a.window)  // stages that the last nodes do not see all of
-      for (; t < min(t1, ct.tiles - 1) && ct.lo + t * SK < ct.len + NODES - a.window; ++t) turn(std::integral_constant<int, 1>(), t);
+    if (a.window && t == 0 && t < min(t1, ct.tiles - 1)) turn(std::integral_constant<int, 1>(), t++);
     for (; t < min(t1, ct.full); ++t) turn(std::integral_constant<int, 0>(), t);
-    for (; t < min(t1, ct.tiles - 1); ++t) turn(std::integral_constant<int, 1>(), t);
+    if (t < min(t1, ct.tiles - 1)) turn(std::integral_constant<int, 3>(), t++);
     if (t < t1) turn(std::integral_constant<int, 2>(), t);
+    for (int own = 0; own < 2; ++own) {
+      const uint64_t ill = ((uint64_t)bad[own][1] << 32 | bad[own][0]) & (KT == 64 ? ~0ull : 0xffffffffull << (wk * KT));
+      for (uint64_t w = ill; w; w &= w - 1) {
+        const int key = __builtin_ctzll(w), i = own ? ct.full * SK + key : key;  // of the context, behind ct.lo
+        const bool node = own && key >= joint;
+        if (!own && ct.lo + i >= ct.len) break;
+        const bf16_t* const v = (node ? nv + (long)(key - joint) * a.ldq : vc + (long)i * D) + 4 * g;
+        const uint8_t* const v8 = (const uint8_t*)a.vc + head + ((long)ct.lo + i) * D + 4 * g;
+        const float sc = KV8 && !own ? a.vsc[pair_at * a.SmaxP + ct.lo + i] : 1.f;
+#pragma unroll
+        for (int u = 0; u < RT; ++u)
+          if (own ? sees[u] >> key & 1 : ct.lo + i >= from[u])
+#pragma unroll
+            for (int c = 0; c < DT; ++c) {
+              const uint32_t four = KV8 && !own ? *(const uint32_t*)(v8 + 16 * c) : 0;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float f = KV8 && !own ? fp8_at(four, e) * sc : bf2f(v[16 * c + e]);
+                if (!(fabsf(f) < INFINITY)) o[u][c][e] += f;
+              }
+              asm volatile("" ::: "memory");  // this is seldom reached: few registers, not many loads at once
+            }
+      }
+    }
 #pragma unroll
     for (int u = 0; u < RT; ++u) l[u] = over_groups(l[u], [](float p, float q) { return p + q; });
     if constexpr (WK > 1) {  // the keys' shares, joined in order

@@ -125,6 +125,51 @@ def test_attention_keeps_windows_apart(bad):
     assert not torch.isfinite(of[:, :, 5]).any() and torch.isfinite(of[:, :, :5]).all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 2, 128), (8, 2, 128), (8, 1, 128), (32, 1, 128), (4, 4, 64), (32, 2, 64), (3, 1, 32)])
+def test_attention_windows_part_way_down_the_context(Hq, Hkv, D, fp8, bad):
+    """the same far from its end, where a window of 100 starts: a value, or in e4m3 its scale, and what key and value hold before it"""
+    if fp8 and D != 128:
+        pytest.skip("an e4m3 cache has heads of 128")
+    N, window, n = 9, 100, 300  # node i at position n + i sees the slots from n + i - 99
+    at = n - 95                 # seen by nodes 0 to 4
+    qkv, kc, vc = _rand(N, (Hq + 2 * Hkv) * D), _rand(1, Hkv, 310, D, seed=1), _rand(1, Hkv, 310, D, seed=2)
+    tree, scales = ops.draft_tree(_i32([[-1] + list(range(N - 1))])), {}
+    if fp8:
+        (kc, ks), (vc, vs) = ops.kv_quantize_rows(kc, True), ops.kv_quantize_rows(vc, False)
+        scales = dict(k_scale=torch.nn.functional.pad(ks, (0, 2)), v_scale=torch.nn.functional.pad(vs, (0, 2)))
+    run = lambda: ops.tree_attention(qkv, kc, vc, _i32([n]), tree, Hq, window=window, **scales)
+    want = run()
+    if fp8 and not math.isnan(bad):
+        scales["v_scale"][0, :, at] = bad
+        ill = slice(0, D)
+    else:
+        vc[0, :, at, 5] = 0x7f if fp8 else bad
+        ill = slice(5, 6)
+    got = run()
+    assert torch.equal(got[5:], want[5:])
+    of, ref = got[:5].view(5, Hq, D), want[:5].view(5, Hq, D)
+    assert not torch.isfinite(of[:, :, ill]).any() and (math.isnan(bad) or fp8 or (of[:, :, ill] == bad).all())
+    of[:, :, ill] = ref[:, :, ill]
+    assert torch.equal(of, ref)
+    (scales["k_scale"] if fp8 else kc)[0, :, at] = bad  # scores that are no numbers
+    assert torch.equal(run()[5:], want[5:])
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,N,n", [(8, 2, 128, 64, 70), (2, 2, 128, 5, 127), (4, 4, 64, 30, 63), (3, 1, 32, 9, 20)])
+def test_attention_infinite_value_at_the_end_of_the_context(Hq, Hkv, D, N, n):
+    """the last slot's value stands in for keys behind it: infinite it is infinite in every node's sum, and no NaN"""
+    qkv, kc, vc = _rand(N, (Hq + 2 * Hkv) * D), _rand(1, Hkv, n + 3, D, seed=1), _rand(1, Hkv, n + 3, D, seed=2)
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))]))
+    want = ops.tree_attention(qkv, kc, vc, _i32([n]), tree, Hq).view(N, Hq, D)
+    vc[0, :, n - 1, 7] = math.inf
+    got = ops.tree_attention(qkv, kc, vc, _i32([n]), tree, Hq).view(N, Hq, D)
+    assert (got[:, :, 7] == math.inf).all()
+    got[:, :, 7] = want[:, :, 7]
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("lens", [[2100], [1500, 9, 700]])
 @pytest.mark.parametrize("N", [2, 30])
 def test_attention_long(lens, N):
