@@ -61,6 +61,11 @@ bool apart(const Tensor& a, const Tensor& b) {
   return col >= b.size(1) && col + a.size(1) <= pitch;
 }
 
+bool shares(const Tensor& a, const Tensor& b) {
+  const auto s = at::get_overlap_status(a, b);
+  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+}
+
 // the slots' scales of an e4m3 cache [.., rows, heads, slots, 128], alike for keys and values
 struct Scales { float* k = nullptr; float* v = nullptr; long layer = 0; int slots = 0; };
 Scales scales(const Tensor& kc, const optional<Tensor>& k, const optional<Tensor>& v) {
@@ -114,6 +119,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   TORCH_CHECK_VALUE(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && (qkv.stride(1) == 1 || qkv.size(0) == 0),
                     "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim] expected, got ", qkv.sizes(), ", ", kc.sizes());
   const int64_t B = kc.size(0), Hkv = kc.size(1), Smax = kc.size(2), D = kc.size(3), N = see.size(1);
+  TORCH_CHECK_VALUE(N >= 1 && N <= 64, "tree_attention: 1 to 64 nodes a row expected, got a tree ", see.sizes());
   const Scales sc = scales(kc, k_scale, v_scale);
   TORCH_CHECK_VALUE(sc.k ? qkv.scalar_type() == at::kBFloat16 : kc.scalar_type() == qkv.scalar_type(), "caches of ", kc.scalar_type(),
                     " under queries of ", qkv.scalar_type());
@@ -135,7 +141,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   TORCH_CHECK_VALUE(out.scalar_type() == qkv.scalar_type() && out.dim() == 2 && out.size(0) == B * N && out.size(1) == Hq * D &&
                         (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
   at::assert_no_internal_overlap(out);
-  TORCH_CHECK_VALUE(apart(out, qkv), "tree_attention: out overlaps qkv");
+  TORCH_CHECK_VALUE(apart(out, qkv) && !shares(out, kc) && !shares(out, vc), "tree_attention: out overlaps what is read");
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window) : 0;
   TORCH_CHECK_VALUE(S || !sc.k || !B, "tree_attention: an e4m3 cache of this size");
@@ -159,10 +165,12 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
   TORCH_CHECK_VALUE(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
               "tree_accept: caches [layers, rows, heads, slots, dim] and rows of every layer (256 at most)");
   const int64_t L = kc.size(0), B = kc.size(1), Hkv = kc.size(2), Smax = kc.size(3), D = kc.size(4), N = see.size(1);
+  TORCH_CHECK_VALUE(N >= 1 && N <= 64, "tree_accept: 1 to 64 nodes a row expected, got a tree ", see.sizes());
   on(vc, kc, "tree_accept v_cache");
   TORCH_CHECK_VALUE(D > 0 && Hkv > 0, "tree_accept: caches of no heads");
   TORCH_CHECK_VALUE(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
               "tree_accept: caches of one type and layout, contiguous in each layer");
+  TORCH_CHECK_VALUE(!shares(kc, vc), "tree_accept: keys and values of one memory");
   const Scales sc = scales(kc, k_scale, v_scale);
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
@@ -240,6 +248,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> token_alternatives(const Tensor& logi
   act(logits, "logits");
   TORCH_CHECK_VALUE(logits.dim() == 2 && top >= 1 && top <= 32 && top <= logits.size(1) && logits.size(1) < (1L << 30),
                     "1 to 32 alternatives of logits [tokens, vocabulary] expected: ", top, " of ", logits.sizes());
+  TORCH_CHECK_VALUE(logits.size(0) < (1L << 22), "token_alternatives: ", logits.size(0), " rows");  // of up to 1024 threads each in a launch
   TORCH_CHECK_VALUE((float)c > 0 && std::isfinite((float)c), "inverse temperature ", c);
   const Tensor x = logits.stride(1) == 1 || logits.size(1) == 1 ? logits : logits.contiguous();
   optional<Tensor> t;

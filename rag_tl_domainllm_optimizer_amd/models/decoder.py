@@ -481,8 +481,9 @@ class CausalLM(nn.Module):
         cfg = self.cfg
         kv8 = getattr(cache, "fp8", False)
         cos, sin = self.rope(tokens.device)
-        pos = tree.pos.reshape(-1)
-        x = self.embed_tokens(tokens.reshape(-1), pos)
+        # what is no node may hold any token (an idle row's next one is -1), and a tree may reach past the positions that there are
+        pos = tree.pos.reshape(-1).clamp(0, cfg.max_position - 1)
+        x = self.embed_tokens(torch.where(tree.see != 0, tokens, 0).reshape(-1), pos)
         residual, drafts = None, []
         for li, layer in enumerate(self.layers):
             qkv, residual, rotated = layer.attn_in_rope(x, residual, (pos, cos, sin) if cos is not None else None)

@@ -51,6 +51,11 @@ def _scales(k_cache, v_cache, k_scale, v_scale) -> bool:
     return fp8
 
 
+def _nodes(tree):
+    if tree.see.dim() != 2 or not 1 <= tree.see.shape[1] <= MAX_NODES:
+        raise ValueError(f"a tree [rows, 1 .. {MAX_NODES} nodes] expected, got {tuple(tree.shape)}")
+
+
 def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0: Optional[torch.Tensor] = None) -> DraftTree:
     """The plan of drafted trees: ``parent`` int32 [rows, nodes <= 64] holds an earlier node of the row for each (anything else: none, a tree of its
     own), ``nodes`` int32 [rows] how many of a row's are nodes (0: the row idles; default all), ``pos0`` int32 [rows] the position
@@ -79,6 +84,7 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    _nodes(tree)
     B, Hkv, Smax, D = k_cache.shape
     N = tree.shape[1]
     if tree.shape[0] != B or qkv.dim() != 2 or qkv.shape[0] != B * N:
@@ -113,6 +119,7 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
         return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale)
     if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    _nodes(tree)
     L, B, Hkv, Smax, D = k_cache.shape
     if tree.shape[0] != B or tuple(tokens.shape) != tuple(tree.shape) or tuple(choice.shape) != tuple(tree.shape):
         raise ValueError(f"tree {tuple(tree.shape)}, tokens {tuple(tokens.shape)} and choice {tuple(choice.shape)} of {B} rows do not go together")

@@ -140,6 +140,9 @@ def test_alternatives_of_masked_rows_have_finite_gradients():
     lambda: _accept(drafts=[torch.zeros(6, 16)] * 2),
     lambda: _accept(drafts=[torch.zeros(6, 32, dtype=torch.bfloat16)] * 2),
     lambda: _accept(kv_len=torch.zeros(1, dtype=torch.int32)),
+    lambda: _attend(tree=_empty(2, 0), qkv=torch.zeros(0, 32)),
+    lambda: _attend(tree=_empty(2, 65), qkv=torch.zeros(130, 32)),
+    lambda: _accept(tree=_empty(2, 0), tokens=torch.zeros(2, 0, dtype=torch.int64), choice=torch.zeros(2, 0, dtype=torch.int64), drafts=[torch.zeros(0, 32)] * 2),
     lambda: ops.token_alternatives(torch.zeros(3, 8), None, 0),
     lambda: ops.token_alternatives(torch.zeros(3, 8), None, 9),
     lambda: ops.token_alternatives(torch.zeros(3, 80), None, 33),
@@ -154,17 +157,21 @@ def test_refused(bad):
         bad()
 
 
-def _attend(qkv=None, kc=None, kv_len=None, kv_start=None, Hq=4, window=0, scale=None):
+def _empty(*shape):
+    return ops.DraftTree(*(torch.zeros(*shape, dtype=t) for t in (torch.int32, torch.int64, torch.int32)))
+
+
+def _attend(qkv=None, kc=None, kv_len=None, kv_start=None, Hq=4, window=0, scale=None, tree=None):
     z = torch.zeros
     kc = z(2, 2, 9, 4) if kc is None else kc
     return ops.tree_attention(z(6, 32) if qkv is None else qkv, kc, kc, z(2, dtype=torch.int32) if kv_len is None else kv_len,
-                              _tree([[-1, 0, 0]] * 2), Hq, kv_start, window, scale)
+                              _tree([[-1, 0, 0]] * 2) if tree is None else tree, Hq, kv_start, window, scale)
 
 
-def _accept(tokens=None, choice=None, drafts=None, kv_len=None):
+def _accept(tokens=None, choice=None, drafts=None, kv_len=None, tree=None):
     ids = torch.zeros(2, 3, dtype=torch.int64)
     kc = torch.zeros(2, 2, 2, 9, 4)
-    return ops.tree_accept(_tree([[-1, 0, 0]] * 2), ids if tokens is None else tokens, ids if choice is None else choice,
+    return ops.tree_accept(_tree([[-1, 0, 0]] * 2) if tree is None else tree, ids if tokens is None else tokens, ids if choice is None else choice,
                            [torch.zeros(6, 32)] * 2 if drafts is None else drafts, kc, kc.clone(),
                            torch.zeros(2, dtype=torch.int32) if kv_len is None else kv_len)
 
@@ -211,6 +218,27 @@ def test_answers_written_by_drafts_are_the_greedy_ones(preset):
         steps += 1
     assert [x[:24] for x in got] == want
     assert steps < 20
+
+
+@pytest.mark.parametrize("preset", ["tiny-mistral", "tiny-opt"])
+def test_verify_of_idle_rows_and_of_trees_past_the_last_position(preset):
+    """an idle row's next token is -1; nodes past the model's positions leave those before them as they are"""
+    cfg = models.resolve_preset(preset)
+    m = models.CausalLM(cfg, dtype=torch.float32, seed=3)
+    B, N, S = 3, 6, cfg.max_position
+    cache = KVCache(cfg.num_layers, B, cfg.num_kv_heads, S, cfg.head_dim, "cpu", torch.float32)
+    cache.k.normal_(), cache.v.normal_()
+    kv_len = torch.tensor([9, 0, S - 3], dtype=torch.int32)
+    chain = torch.tensor([[-1] + list(range(N - 1))] * B, dtype=torch.int32)
+    tokens = torch.arange(3, 3 + B * N).view(B, N)
+    idle = tokens.clone()
+    idle[1] = -1
+    h, drafts = m.verify(idle, ops.draft_tree(chain, torch.tensor([N, 0, N], dtype=torch.int32), kv_len), kv_len, None, cache)
+    fit = torch.tensor([N, 0, 3], dtype=torch.int32)
+    tree = ops.draft_tree(chain, fit, kv_len)
+    want, _ = m.verify(tokens, tree, kv_len, None, cache)
+    for b, n in enumerate(fit.tolist()):
+        assert torch.allclose(h.view(B, N, -1)[b, :n], want.view(B, N, -1)[b, :n], rtol=1e-5, atol=1e-6)
 
 
 def _depth(up, i):

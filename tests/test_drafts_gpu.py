@@ -637,6 +637,14 @@ def test_runs_repeat_bit_by_bit():
     lambda: ops.tree_attention(_rand(2, 512), _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4,
                                out=torch.empty(1, 256, dtype=BF16, device=DEV).expand(2, 256)),
     lambda: _in_place(_rand(2, 512)),
+    lambda: _over_the_cache(_rand(1, 2, 9, 64)),
+    lambda: ops.tree_attention(_rand(0, 512), _rand(2, 2, 9, 64), _rand(2, 2, 9, 64), _i32([3, 3]), _empty(2, 0), 4),
+    lambda: ops.tree_attention(_rand(130, 512), _rand(2, 2, 9, 64), _rand(2, 2, 9, 64), _i32([3, 3]), _empty(2, 65), 4),
+    lambda: ops.tree_accept(_empty(2, 0), *(torch.zeros(2, 0, dtype=torch.long, device=DEV) for _ in "tc"), [_rand(0, 512)],
+                            *(_rand(1, 2, 2, 9, 64) for _ in "kv"), _i32([3, 3])),
+    lambda: ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.long, device=DEV) for _ in "tc"), [_rand(2, 512)],
+                            *[_rand(1, 1, 2, 9, 64)] * 2, _i32([3])),
+    lambda: ops.token_alternatives(_rand(1, 1).expand(1 << 22, 1), None, 1),
     lambda: ops.tree_attention(_rand(2, 512, dtype=F32), *(torch.zeros(1, 1, 9, 128, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]),
                                ops.draft_tree(_i32([[-1, 0]])), 2, k_scale=torch.ones(1, 1, 9, device=DEV), v_scale=torch.ones(1, 1, 9, device=DEV)),
     lambda: ops.tree_attention(_rand(2, 512), *(torch.zeros(1, 1, 9, 128, dtype=torch.uint8, device=DEV) for _ in "kv"), _i32([3]),
@@ -657,8 +665,37 @@ def test_refused(bad):
         bad()
 
 
+def _empty(*shape):
+    return ops.DraftTree(*(torch.zeros(*shape, dtype=t, device=DEV) for t in (torch.int32, torch.int64, torch.int32)))
+
+
+def _over_the_cache(kc):
+    return ops.tree_attention(_rand(2, 512), kc, _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, out=kc.view(-1)[:512].view(2, 256))
+
+
 def _in_place(qkv):
     return ops.tree_attention(qkv, _rand(1, 2, 9, 64), _rand(1, 2, 9, 64), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, out=qkv[:, :256])
+
+
+@pytest.mark.parametrize("preset", ["tiny-mistral", "tiny-opt"])
+def test_verify_of_idle_rows_and_of_trees_past_the_last_position(preset):
+    """an idle row's next token is -1; nodes past the model's positions leave those before them as they are"""
+    cfg = models.resolve_preset(preset)
+    m = models.CausalLM(cfg, device=DEV, dtype=BF16, seed=3)
+    B, N, S = 3, 6, cfg.max_position
+    cache = KVCache(cfg.num_layers, B, cfg.num_kv_heads, S, cfg.head_dim, DEV)
+    cache.k.normal_(), cache.v.normal_()
+    kv_len = _i32([9, 0, S - 3])
+    chain, tokens = _i32([[-1] + list(range(N - 1))] * B), torch.arange(3, 3 + B * N, device=DEV).view(B, N)
+    idle = tokens.clone()
+    idle[1] = -1
+    h = m.verify(idle, ops.draft_tree(chain, _i32([N, 0, N]), kv_len), kv_len, None, cache)[0].view(B, N, -1)
+    want = m.verify(tokens, ops.draft_tree(chain, _i32([N, 0, 3]), kv_len), kv_len, None, cache)[0].view(B, N, -1)
+    assert torch.equal(h[0], want[0])
+    # six nodes leave the context's last 61 keys of 64 to a stage of their own where three take them into theirs: p is rounded to bf16 against
+    # another maximum, so the states are apart by roundings of half a step, 16 on their way through two layers as below
+    x, y = h[2, :3].float(), want[2, :3].float()
+    assert (x - y).pow(2).mean().sqrt() <= 16 ** 0.5 * 2 ** -8 * y.pow(2).mean().sqrt()
 
 
 def test_a_model_checks_drafts_like_single_steps():
