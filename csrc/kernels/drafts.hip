@@ -204,6 +204,26 @@ __device__ __forceinline__ void read_pair(uint32_t at, u32x4& x, u32x4& y) {
   asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)" : "=&v"(x), "=&v"(y) : "v"(at), "i"(second) : "memory");
 }
 
+// where 16 bytes c of an e4m3 value lie in its row of a stage: eight keys in turn (4 g .. + 3 and 16 behind these) use all banks
+__device__ __forceinline__ int v8_chunk(int key, int c) { return c ^ ((key >> 1 & 3) | (key >> 2 & 4)); }
+// columns of eight keys' bytes each, of eight chunks of 16 (at: of chunk 0)
+template <int offset>
+__device__ __forceinline__ void read_columns8(uint32_t at, uint2 (&v)[8]) {
+  asm volatile(
+      "ds_read_b64_tr_b8 %0, %8 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %1, %9 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %2, %10 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %3, %11 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %4, %12 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %5, %13 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %6, %14 offset:%16\n\t"
+      "ds_read_b64_tr_b8 %7, %15 offset:%16\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+      : "v"(at), "v"(at ^ 16), "v"(at ^ 32), "v"(at ^ 48), "v"(at ^ 64), "v"(at ^ 80), "v"(at ^ 96), "v"(at ^ 112), "i"(offset)
+      : "memory");
+}
+
 // e4m3 byte e of four
 __device__ __forceinline__ float fp8_at(uint32_t four, int e) {
   typedef __attribute__((ext_vector_type(2))) float f32x2_t;
@@ -211,12 +231,12 @@ __device__ __forceinline__ float fp8_at(uint32_t four, int e) {
   return f[e & 1];
 }
 
-// The bound: 128 registers, for two workgroups of eight waves in a CU (e4m3, rows of 128 queries, when it took 162: 91 us, and 81 with the bound).
+// The bound: 128 registers, for two workgroups of eight waves in a CU (in e4m3, with 162: rows of 128 queries 91 us, with the bound 81).
 template <int D, int RT, int WR, int WK, int KT, bool KV8>
 __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
   static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
-  __shared__ __attribute__((aligned(16))) char smem[4 * KB];
+  __shared__ __attribute__((aligned(128))) char smem[4 * KB];
   __shared__ __attribute__((aligned(16))) float scales[KV8 ? 4 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
   __shared__ unsigned bad[2][2];  // keys of the first stage, and of the nodes', whose values are not all numbers
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, r16 = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
@@ -318,47 +338,52 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
         }
       }
     };
-    // An e4m3 cache: two stages are on their way to LDS as they are, in the second half of the buffers; a stage is made bf16 (exact) in the
-    // first half when its turn comes. The nodes' stage, in bf16, takes the second half once the last of these has left it. Measured against
-    // the next stage's bytes in registers, and against a cache in bf16: 64 rows of 48 nodes over 100 to 700 keys in 32 key heads of one
-    // query each 117 -> 77 us (bf16 93), 48 rows of 16 nodes over 150 to 1200 keys in 8 heads of four 45 -> 39 (29), 64 rows of 64 nodes over
-    // 1000 to 4000 keys 246 -> 231 (213): half the bytes, but a pass over LDS and a barrier for them, so it wins where memory bounds the bf16 form.
+    // An e4m3 cache: its stages go to LDS as they are, in a ring of four, three under way, and become bf16 (exact) where fragments are read.
+    // The nodes' stage, in bf16, takes the half of the ring that the last of these is not in. Measured against a cache in bf16: 64 rows of 48 nodes
+    // over 100 to 700 keys in 32 key heads of one query each 73 us for 93, 16 rows of 32 nodes 41 for 46, where memory bounds these; 48 rows of 16 nodes in
+    // 8 heads of four 35 for 29, and 64 rows of 64 nodes over 1000 to 4000 keys 234 for 207, where the instructions do: each wave converts what it
+    // reads. (Converted once, in a pass over LDS with a barrier: 77, 49, 38, 230.)
     const int raw_end = min(t1, ct.tiles - 1);
     auto fetch = [&](int tile) {
-      const int last = ct.len - ct.lo - tile * SK - 1, slot = tile - t0;
+      const int last = ct.len - ct.lo - tile * SK - 1, slot = tile - t0 & 3;
       const long at = head + ((long)ct.lo + (long)tile * SK) * D;
-      char* const dst = smem + 2 * KB + (slot & 1) * KB + wid * 1024;
+      char* const dst = smem + slot * KB + wid * 1024;
 #pragma unroll
       for (int j = 0; j < NJ / 2; ++j) {
-        const int e = (j * NW + wid) * 64 + lane;
-        const uint32_t from = min(e / 8, last) * D + e % 8 * 16;
-        paged::lds_dma16((const char*)a.kc + at, from, dst + j * NW * 1024);
-        paged::lds_dma16((const char*)a.vc + at, from, dst + KB / 2 + j * NW * 1024);
+        const int e = (j * NW + wid) * 64 + lane, key = e / 8;
+        const uint32_t row = min(key, last) * D;
+        paged::lds_dma16((const char*)a.kc + at, row + 16 * paged::kq_chunk<64>(key, e % 8), dst + j * NW * 1024);
+        paged::lds_dma16((const char*)a.vc + at, row + 16 * v8_chunk(key, e % 8), dst + KB / 2 + j * NW * 1024);
       }
       const long sc = pair_at * a.SmaxP + ct.lo + tile * SK;
-      paged::lds_dma4(a.ksc + sc, 4 * min(lane, last), scales[slot & 3]);  // by every wave: the same to the same place
-      paged::lds_dma4(a.vsc + sc, 4 * min(lane, last), scales[slot & 3] + SK);
+      paged::lds_dma4(a.ksc + sc, 4 * min(lane, last), scales[slot]);  // by every wave: the same to the same place
+      paged::lds_dma4(a.vsc + sc, 4 * min(lane, last), scales[slot] + SK);
     };
     constexpr int RAW_LOADS = NJ / 2 * 2 + 2;
-    auto convert = [&](int tile) {
-      const char* const raw = smem + 2 * KB + (tile - t0 & 1) * KB;
-#pragma unroll
-      for (int j = 0; j < SK * D / 16 / (64 * NW); ++j) {
-        // 16 bytes h of a key: elements 8 (4 s + h / 2) .. + 7 of s = 2 (h % 2) and the next; of a value 16 h .. 16 h + 15
-        const int e = j * 64 * NW + tid, key = e / 8, h = e % 8, c = 8 * (h % 2) + h / 2;
-        const uint4 k = *(const uint4*)(raw + 16 * e), v = *(const uint4*)(raw + KB / 2 + 16 * e);
-        *(bf16x8*)(smem + paged::kq_off<D>(key, c)) = fp8x8_to_bf16(k.x, k.y);
-        *(bf16x8*)(smem + paged::kq_off<D>(key, c + 4)) = fp8x8_to_bf16(k.z, k.w);
-        *(bf16x8*)(smem + KB + paged::vv_off<D>(key, 2 * h)) = fp8x8_to_bf16(v.x, v.y);
-        *(bf16x8*)(smem + KB + paged::vv_off<D>(key, 2 * h + 1)) = fp8x8_to_bf16(v.z, v.w);
-      }
-    };
     if (tid < 4) bad[tid / 2][tid & 1] = 0;
-    if (KV8 && t0 < raw_end) {
+    // The queries are waited for here, once, behind the first stages (in each branch, where the compiler can count what is behind them). It does
+    // not know what the turns wait for, and would put waits for all loads, the next stage's among them, in front of every product with them.
+    auto have_queries = [&] {
+#pragma unroll
+      for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int d = 0; d < DS; ++d) asm volatile("" : "+v"(qf[u][d]));
+    };
+    if (KV8 && t0 + 2 < raw_end) {
       fetch(t0);
-      if (t0 + 1 < raw_end) fetch(t0 + 1);
+      fetch(t0 + 1);
+      fetch(t0 + 2);
+      have_queries();
+    } else if (KV8 && t0 + 1 < raw_end) {
+      fetch(t0);
+      fetch(t0 + 1);
+      have_queries();
+    } else if (KV8 && t0 < raw_end) {
+      fetch(t0);
+      have_queries();
     } else {
       stage(t0, KV8);
+      have_queries();
     }
     int cur = KV8;
     // a stage that lies in LDS; MODE 0: every row sees all of its keys, 1: a window leaves out keys of the context for some, 2: the nodes'
@@ -366,13 +391,27 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
     auto multiply = [&](auto mode, int t, char* image) {
       constexpr int MODE = decltype(mode)::value;
       constexpr bool SCALED = KV8 && MODE != 2;
-      char* const Ks = image + wk * KT * D * 2;
-      char* const Vs = Ks + KB;
+      char* const Ks = image + wk * KT * D * (SCALED ? 1 : 2);
+      char* const Vs = Ks + (SCALED ? KB / 2 : KB);
       f32x4 st[KS][RT];
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int u = 0; u < RT; ++u) st[k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int d = 0; d < DS; d += 2) {  // 16 bytes: this lane's eight elements of d and of d + 1
+            const u32x4 w = *(const u32x4*)(Ks + paged::kq_off<64>(16 * k + r16, 2 * g + d / 2));
+            const bf16x8 k0 = fp8x8_to_bf16(w[0], w[1]), k1 = fp8x8_to_bf16(w[2], w[3]);
+#pragma unroll
+            for (int u = 0; u < RT; ++u) {
+              st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, qf[u][d], st[k][u], 0, 0, 0);
+              st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, qf[u][d + 1], st[k][u], 0, 0, 0);
+            }
+          }
+      } else {
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -382,6 +421,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
 #pragma unroll
           for (int u = 0; u < RT; ++u) st[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[u][d], st[k][u], 0, 0, 0);
         }
+      }
       const int key0 = wk * KT + 4 * g;  // of the stage: this lane's keys are key0 + 16 k + e
       if constexpr (SCALED) {
 #pragma unroll
@@ -492,6 +532,24 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
         return v;
       };
       const int key_a = 4 * g + (lane >> 2 & 3), pcol = lane & 3;  // transposed reads: rows 16 apart have the same swizzle
+      if constexpr (SCALED) {
+        // lane pairs read the 16 columns of keys 4 g .. + 3 and 16 behind these; the lane gets its column of the eight
+        const int q = lane >> 1 & 7, key = 4 * g + (q & 3) + 16 * (q >> 2);
+        const uint32_t at = lds_addr(Vs + key * D + 16 * v8_chunk(key, 0) + 8 * (lane & 1));
+#pragma unroll
+        for (int h = 0; h < KT / 32; ++h) {
+          uint2 v[8];
+          if (h == 0) read_columns8<0>(at, v);
+          else read_columns8<32 * D>(at, v);
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            const bf16x8 vf = of_keys(fp8x8_to_bf16(v[c & 7].x, v[c & 7].y), h);
+#pragma unroll
+            for (int u = 0; u < RT; ++u) o[u][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[h][u], o[u][c], 0, 0, 0);
+          }
+        }
+        return;
+      }
 #pragma unroll
       for (int c = 0; c < DT; c += 4) {
         uint32_t va[4];
@@ -524,42 +582,50 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
     // The values of a stage that some row does not see all of: 0 times what is no number is none, so such values count as 0 in the product and
     // are added at the end for the rows that see them. These are the nodes' stage and, with a window, the first one (the last node's starts less
     // than NODES keys behind the first one's). The reads are of this kind because ordinary ones would wait for the next stage.
-    auto only_numbers = [&](char* values, bool own) {
-      constexpr int second = KB / 2;
+    auto only_numbers = [&](char* values, auto own) {
+      constexpr bool raw = KV8 && !own.value;
+      constexpr int second = raw ? KB / 4 : KB / 2;
 #pragma unroll 1
       for (int e = 16 * tid; e < second; e += 16 * 64 * NW) {
         u32x4 w[2];
         read_pair<second>(lds_addr(values + e), w[0], w[1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int key = (e + h * second) / (2 * D);
+          const int key = (e + h * second) / (raw ? D : 2 * D);
           u32x4 x = w[h];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] &= ((x[i] & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((x[i] & 0x7f800000u) == 0x7f800000u ? 0xffffu : ~0u);
+          for (int i = 0; i < 4; ++i) {
+            if (raw) x[i] &= ~((((x[i] & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu);
+            else x[i] &= ((x[i] & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((x[i] & 0x7f800000u) == 0x7f800000u ? 0xffffu : ~0u);
+          }
           bool ill = x[0] != w[h][0] || x[1] != w[h][1] || x[2] != w[h][2] || x[3] != w[h][3];
           if (ill) *(u32x4*)(values + e + h * second) = x;
-          if (KV8 && !own) ill |= !(fabsf(scales[0][SK + key]) < INFINITY);
-          if (ill) atomicOr(&bad[own][key / 32], 1u << (key % 32));
+          if (raw) ill |= !(fabsf(scales[0][SK + key]) < INFINITY);
+          if (ill) atomicOr(&bad[own.value][key / 32], 1u << (key % 32));
         }
       }
     };
     auto turn = [&](auto mode, int t) {
       constexpr int MODE = decltype(mode)::value;
       if constexpr (KV8 && MODE != 2) {
-        if (t + 1 < raw_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(RAW_LOADS) : "memory");  // this stage, not the next one
+        // this stage, not those behind it
+        if (t + 2 < raw_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * RAW_LOADS) : "memory");
+        else if (t + 1 < raw_end) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(RAW_LOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");  // ... of every wave, and the stage before is multiplied
-        convert(t);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        asm volatile("s_barrier" ::: "memory");
+        const int slot = t - t0 & 3;
         if constexpr (MODE == 1) {
-          only_numbers(smem + KB, false);
+          only_numbers(smem + slot * KB + KB / 2, std::false_type());
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           asm volatile("s_barrier" ::: "memory");
         }
-        if (t + 2 < raw_end) fetch(t + 2);
-        else if (t + 2 == ct.tiles && t + 1 < t1) stage(t + 1, 1);
-        if (row0 < M) multiply(mode, t, smem);
+        if (t + 3 < raw_end) {
+          fetch(t + 3);
+        } else if (t + 1 == raw_end && raw_end < t1) {
+          cur = slot < 2;
+          stage(t + 1, cur);
+        }
+        if (row0 < M) multiply(mode, t, smem + slot * KB);
         return;
       }
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // this stage, issued one ago
@@ -568,7 +634,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kerne
       char* const image = smem + 2 * cur * KB;
       cur ^= 1;
       if constexpr (MODE == 1 || MODE == 2) {
-        only_numbers(image + KB, MODE == 2);
+        only_numbers(image + KB, std::bool_constant<MODE == 2>());
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         asm volatile("s_barrier" ::: "memory");
       }
