@@ -231,9 +231,11 @@ __device__ __forceinline__ float fp8_at(uint32_t four, int e) {
   return f[e & 1];
 }
 
-// The bound: 128 registers, for two workgroups of eight waves in a CU (in e4m3, with 162: rows of 128 queries 91 us, with the bound 81).
+// The bound: 128 registers where two workgroups of eight waves share a CU (in e4m3, with 162: rows of 128 queries 91 us, with the bound 81); elsewhere 256,
+// without which the compiler keeps some in the matrix cores' file and moves them in each stage (32 rows of 5 nodes, 12 heads of 64: 11.3 us, with
+// it 10.7; 64 rows of 64 nodes 209 and 205).
 template <int D, int RT, int WR, int WK, int KT, bool KV8>
-__global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 1) void tree_mfma_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
   static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
   __shared__ __attribute__((aligned(128))) char smem[4 * KB];
