@@ -342,8 +342,8 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
     };
     // An e4m3 cache: its stages go to LDS as they are, in a ring of four, three under way, and become bf16 (exact) where fragments are read.
     // The nodes' stage, in bf16, takes the half of the ring that the last of these is not in. Measured against a cache in bf16: 64 rows of 48 nodes
-    // over 100 to 700 keys in 32 key heads of one query each 73 us for 93, 16 rows of 32 nodes 41 for 46, where memory bounds these; 48 rows of 16 nodes in
-    // 8 heads of four 35 for 29, and 64 rows of 64 nodes over 1000 to 4000 keys 234 for 207, where the instructions do: each wave converts what it
+    // over 100 to 700 keys in 32 key heads of one query each 74 us for 93, 16 rows of 32 nodes 37 for 46, where memory bounds these; 48 rows of 16 nodes in
+    // 8 heads of four 35 for 29, and 64 rows of 64 nodes over 1000 to 4000 keys 233 for 204, where the instructions do: each wave converts what it
     // reads. (Converted once, in a pass over LDS with a barrier: 77, 49, 38, 230.)
     const int raw_end = min(t1, ct.tiles - 1);
     auto fetch = [&](int tile) {
