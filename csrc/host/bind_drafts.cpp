@@ -159,7 +159,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
 
 std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens_, const Tensor& choice_,
                                                const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len_,
-                                               const optional<Tensor>& k_scale, const optional<Tensor>& v_scale) {
+                                               const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, int64_t heads) {
   if (!has(k_scale)) act(kc, "tree_accept k_cache");
   TORCH_CHECK_VALUE(kc.is_cuda(), "tree_accept k_cache: GPU tensor expected");
   TORCH_CHECK_VALUE(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
@@ -176,20 +176,24 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
   whole(see, at::kLong, {B, N}, kc, "tree_accept tree");
   const Tensor tokens = ints(tokens_, at::kLong, {B, N}, kc, "tokens"), choice = ints(choice_, at::kLong, {B, N}, kc, "choice");
-  std::vector<const void*> at;
-  std::vector<Tensor> held;  // e4m3: rows at 16 bytes, others are copied
-  const bool copy = sc.k && std::any_of(drafts.begin(), drafts.end(), [](const Tensor& x) { return x.dim() != 2 || !al(x, 16) || x.stride(0) % 8; });
-  if (copy)
-    for (const Tensor& x : drafts) held.push_back(x.clone(at::MemoryFormat::Contiguous));
-  const std::vector<Tensor>& rows = copy ? held : drafts;
-  for (const Tensor& x : rows) {
+  bool copy = false;  // e4m3: rows at 16 bytes, others are copied
+  for (const Tensor& x : drafts) {
     on(x, kc, "tree_accept drafts");
-    TORCH_CHECK_VALUE(x.scalar_type() == (sc.k ? at::kBFloat16 : kc.scalar_type()) && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == rows[0].sizes() &&
-                    x.stride(0) == rows[0].stride(0) && x.size(0) == B * N && x.size(1) % D == 0 && x.size(1) / D > 2 * Hkv,
+    TORCH_CHECK_VALUE(x.scalar_type() == (sc.k ? at::kBFloat16 : kc.scalar_type()) && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
+                    x.stride(0) == drafts[0].stride(0) && x.size(0) == B * N,
                 "tree_accept: drafts [rows nodes, (heads + 2 key heads) dim] of the caches' type, alike in every layer");
-    at.push_back(x.data_ptr());
+    copy = copy || (sc.k && (!al(x, 16) || x.stride(0) % 8));
   }
-  const int64_t Hq = rows[0].size(1) / D - 2 * Hkv;
+  // keys lie behind `heads` queries; where nobody said how many (0), the rows hold nothing behind [q | k | v]
+  const int64_t cols = drafts[0].size(1), Hq = heads ? heads : cols / D - 2 * Hkv;
+  TORCH_CHECK_VALUE(Hq > 0 && Hq % Hkv == 0 && Hq < 65536 && cols >= (Hq + 2 * Hkv) * D && (heads || cols % D == 0), "tree_accept: ", Hq,
+                    " heads over ", Hkv, " of ", D, " do not fit drafts of ", cols, " columns");
+  std::vector<const void*> at;
+  std::vector<Tensor> held;
+  if (copy)
+    for (const Tensor& x : drafts) held.push_back(x.narrow(1, 0, (Hq + 2 * Hkv) * D).clone(at::MemoryFormat::Contiguous));
+  const std::vector<Tensor>& rows = copy ? held : drafts;
+  for (const Tensor& x : rows) at.push_back(x.data_ptr());
   TORCH_CHECK_VALUE(N * Hkv * D < (1L << 30), "tree_accept: sizes");
   const c10::DeviceGuard guard(kc.device());
   Tensor count = at::empty({B}, parent.options()), path = at::empty({B, N}, parent.options()), next = at::empty({B}, tokens.options());

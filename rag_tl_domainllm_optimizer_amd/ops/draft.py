@@ -23,11 +23,12 @@ MAX_NODES = 64  # a node's ancestors are the bits of one word
 @dataclass
 class DraftTree:
     """Trees of a batch, [rows, nodes] each: parent int32 (as given), see int64 (bit j: the node itself or its ancestor j; 0: not
-    a node), pos int32."""
+    a node), pos int32. ``heads``: query heads of the rows that :func:`tree_attention` read with it (0: none yet)."""
 
     parent: torch.Tensor
     see: torch.Tensor
     pos: torch.Tensor
+    heads: int = 0
 
     @property
     def shape(self):
@@ -81,7 +82,9 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     nodes or outside its window, does not reach it, NaN and infinities among it. uint8 caches hold e4m3 (heads of 128), as
     ``kv_quantize_rows`` and decoding write them, with their slots' scales in ``k_scale``, ``v_scale`` [rows, Hkv, >= Smax]."""
     if on_gpu(qkv):
-        return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale)
+        o = native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale)
+        tree.heads = Hq
+        return o
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     _nodes(tree)
@@ -104,19 +107,25 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if fp8:
         k_cache, v_cache = (kv_dequantize(c, sc[..., :Smax], k) for c, sc, k in ((k_cache, k_scale, True), (v_cache, v_scale, False)))
     o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale)
+    tree.heads = Hq
     return o if out is None else out.copy_(o)
 
 
 def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, drafts: List[torch.Tensor], k_cache: torch.Tensor,
-                v_cache: torch.Tensor, kv_len: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+                v_cache: torch.Tensor, kv_len: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                Hq: Optional[int] = None):
     """The path that the model agrees with -> (its length int32 [rows], its nodes int32 [rows, nodes] (-1 behind them), the token after it int64
     [rows]). ``tokens`` / ``choice`` int64 [rows, nodes]: the drafted tokens, and what the model writes after each; the path starts at node 0 and goes
     on with the child whose token is the choice (the first of equal ones). Keys and values of its nodes go from ``drafts``
     (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
     itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out.
-    ``k_scale`` / ``v_scale`` [layers, rows, Hkv, >= Smax]: the caches are fp8, and rows are rounded into them as ``kv_store_fp8`` does."""
+    ``Hq``: query heads in front of the keys in ``drafts``, by default as :func:`tree_attention` read them with this tree; before it did, rows
+    hold nothing behind [q | k | v]. ``k_scale`` / ``v_scale`` [layers, rows, Hkv, >= Smax]: the caches are fp8, and rows are rounded into them as ``kv_store_fp8`` does."""
+    if Hq is not None and Hq < 1:
+        raise ValueError(f"{Hq} query heads")
+    heads = tree.heads if Hq is None else Hq
     if on_gpu(k_cache):
-        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale)
+        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale, heads)
     if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     _nodes(tree)
@@ -129,8 +138,13 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
         raise ValueError("caches of no heads")
     fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
     if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or (x.dtype != k_cache.dtype and not fp8) or x.shape[0] != B * tree.shape[1]
-                               or x.shape[1] % D or x.shape[1] <= 2 * Hkv * D for x in drafts):
+                               for x in drafts):
         raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")
+    cols = drafts[0].shape[1]
+    Hq = heads or cols // D - 2 * Hkv
+    if Hq < 1 or Hq % Hkv or cols < (Hq + 2 * Hkv) * D or (not heads and cols % D):
+        raise ValueError(f"{Hq} heads over {Hkv} of {D} do not fit drafts of {cols} columns")
+    drafts = [x[:, :(Hq + 2 * Hkv) * D] for x in drafts]
     kv_len = _ints(kv_len, "kv_len", (B,), k_cache)
     store = (lambda x, k: kv_quantize_rows(x, k)) if fp8 else None
     return ref.tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, store, k_scale, v_scale)
