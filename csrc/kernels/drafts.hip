@@ -831,13 +831,15 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
     const int64_t tok = in ? a.tokens[at + tid] : 0;
     const uint64_t choice = in ? (uint64_t)a.choice[at + tid] : 0;
     const bool child = see != 0 && p >= 0 && p < tid;
+    const int room = a.Smax - max(a.kv_len[b], 0);
     int cur = 0, n = 0, mine = -1;
     int64_t last = -1;
-    if (__ballot(see != 0) & 1) {
+    if (__ballot(see != 0) & 1 && room > 0) {
       for (;;) {  // nodes along a path rise: at most N steps
         if (tid == n) mine = cur;
         ++n;
         last = (int64_t)lane64(choice, cur);
+        if (n == room) break;  // a node without a slot would be missing from the context of what follows it
         const uint64_t go = __ballot(child && p == cur && tok == last);
         if (!go) break;
         cur = __builtin_ctzll(go);
@@ -851,7 +853,7 @@ __global__ __launch_bounds__(256) void tree_accept_kernel(AcceptArgs a) {
     }
   }
   __syncthreads();
-  const int len = max(a.kv_len[b], 0), n = min(steps, a.Smax - len);  // slots that are there
+  const int len = max(a.kv_len[b], 0), n = steps;
   const U* const x = (const U*)a.drafts[layer] + at * a.ldq;
   if constexpr (KV8) {
     const int c = tid & 15;  // 16 lanes a row

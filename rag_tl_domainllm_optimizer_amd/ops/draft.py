@@ -118,7 +118,8 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
     [rows]). ``tokens`` / ``choice`` int64 [rows, nodes]: the drafted tokens, and what the model writes after each; the path starts at node 0 and goes
     on with the child whose token is the choice (the first of equal ones). Keys and values of its nodes go from ``drafts``
     (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
-    itself is the caller's to advance by the length. An idle row has length 0 and token -1. Slots past the cache are left out.
+    itself is the caller's to advance by the length. An idle row has length 0 and token -1. A path ends
+    with the cache: its last node is the one that took the last slot, the token the choice after that; a row without a slot idles.
     ``Hq``: query heads in front of the keys in ``drafts``, by default as :func:`tree_attention` read them with this tree; before it did, rows
     hold nothing behind [q | k | v]. ``k_scale`` / ``v_scale`` [layers, rows, Hkv, >= Smax]: the caches are fp8, and rows are rounded into them as ``kv_store_fp8`` does."""
     if Hq is not None and Hq < 1:

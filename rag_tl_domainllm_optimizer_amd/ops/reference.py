@@ -446,16 +446,15 @@ def tree_accept(parent, see, tokens, choice, drafts, kc, vc, kv_len, store=None,
     after = torch.full((B,), -1, dtype=torch.int64, device=kc.device)
     up, tok, ch, live = parent.tolist(), tokens.tolist(), choice.tolist(), (see != 0).tolist()
     for b in range(B):
-        nodes, cur = [], 0 if live[b][0] else -1
+        at = max(int(kv_len[b]), 0)
+        nodes, cur = [], 0 if live[b][0] and at < Smax else -1
         while cur >= 0:
             nodes.append(cur)
-            cur = next((i for i in range(cur + 1, N) if live[b][i] and up[b][i] == cur and tok[b][i] == ch[b][cur]), -1)
+            cur = -1 if at + len(nodes) == Smax else next((i for i in range(cur + 1, N) if live[b][i] and up[b][i] == cur and tok[b][i] == ch[b][cur]), -1)
         if not nodes:
             continue
         count[b], after[b] = len(nodes), ch[b][nodes[-1]]
         path[b, :len(nodes)] = torch.tensor(nodes, dtype=torch.int32)
-        at = max(int(kv_len[b]), 0)
-        nodes = nodes[:max(Smax - at, 0)]
         for layer, x in enumerate(drafts):
             rows = x.view(B, N, -1, D)[b, nodes].transpose(0, 1)
             for c, sc, new, k in ((kc, ksc, rows[-2 * Hkv:-Hkv], True), (vc, vsc, rows[-Hkv:], False)):

@@ -35,3 +35,43 @@ def test_accept_refuses_rows_that_do_not_hold_the_heads(cols, Hkv, Hq):
     with pytest.raises(ValueError):
         ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.int64) for _ in "tc"), [torch.zeros(2, cols)],
                         *(torch.zeros(1, 1, Hkv, 9, 4) for _ in "kv"), _i32([3]), Hq=Hq)
+
+
+# ------------------------------------------------------------------------------------------ the end of the cache
+def test_accept_ends_a_path_at_the_end_of_the_cache():
+    """the last node that has a slot ends the path, and the next token is the choice after it; a row without a slot idles"""
+    N, L, Hq, Hkv, D, slots = 6, 2, 2, 1, 4, 20
+    lens = [slots - 8, slots - 6, slots - 5, slots - 1, slots, slots + 9, -3]
+    B = len(lens)
+    tokens = torch.arange(N).repeat(B, 1)
+    choice = torch.cat([tokens[:, 1:], tokens[:, :1] + 77], 1)
+    rows = [torch.randn(B * N, (Hq + 2 * Hkv) * D) for _ in range(L)]
+    kc, vc = (torch.full((L, B, Hkv, slots, D), 3.0) for _ in "kv")
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))] * B))
+    count, path, after = ops.tree_accept(tree, tokens, choice, rows, kc, vc, _i32(lens))
+    want = [6, 6, 5, 1, 0, 0, 6]
+    assert count.tolist() == want
+    assert path.tolist() == [list(range(n)) + [-1] * (N - n) for n in want]
+    assert after.tolist() == [77, 77, 5, 1, -1, -1, 77]
+    for b, n in enumerate(want):
+        at = max(lens[b], 0)
+        for layer in range(L):
+            x = rows[layer].view(B, N, -1, D)[b, :n].transpose(0, 1)
+            for c, new in ((kc, x[Hq:Hq + Hkv]), (vc, x[Hq + Hkv:])):
+                whole = torch.full((Hkv, slots, D), 3.0)
+                whole[:, at:at + n] = new
+                assert torch.equal(c[layer, b], whole)
+
+
+def test_steps_stop_at_the_end_of_the_cache():
+    """the length that a caller advances never passes the cache, however often the step is taken"""
+    N, slots = 4, 10
+    tokens = torch.arange(N)[None]
+    kc, vc = torch.zeros(1, 1, 1, slots, 4), torch.zeros(1, 1, 1, slots, 4)
+    kv_len, counts = _i32([3]), []
+    for _ in range(4):
+        tree = ops.draft_tree(_i32([[-1, 0, 1, 2]]), pos0=kv_len)
+        count, path, after = ops.tree_accept(tree, tokens, (tokens + 1) % N, [torch.randn(N, 12)], kc, vc, kv_len)
+        kv_len = kv_len + count
+        counts.append((int(count), int(after)))
+    assert counts == [(4, 0), (3, 3), (0, -1), (0, -1)] and int(kv_len) == slots

@@ -105,3 +105,35 @@ def test_accept_refuses_rows_that_do_not_hold_the_heads(cols, Hkv, Hq):
     with pytest.raises(ValueError):
         ops.tree_accept(ops.draft_tree(_i32([[-1, 0]])), *(torch.zeros(1, 2, dtype=torch.int64, device=DEV) for _ in "tc"), [_rand(2, cols)],
                         *(_rand(1, 1, Hkv, 9, 4) for _ in "kv"), _i32([3]), Hq=Hq)
+
+
+# ------------------------------------------------------------------------------------------ the end of the cache
+@pytest.mark.parametrize("D,dtype,fp8", [(128, BF16, False), (128, BF16, True), (6, BF16, False), (20, F32, False)])
+def test_accept_ends_a_path_at_the_end_of_the_cache(D, dtype, fp8):
+    """the last node that has a slot ends the path, and the next token is the choice after it; a row without a slot idles"""
+    N, L, Hq, Hkv, slots = 6, 2, 2, 1, 20
+    lens = [slots - 8, slots - 6, slots - 5, slots - 1, slots, slots + 9, -3]
+    B = len(lens)
+    tokens = torch.arange(N, device=DEV).repeat(B, 1)
+    choice = torch.cat([tokens[:, 1:], tokens[:, :1] + 77], 1)
+    rows = [_rand(B * N, (Hq + 2 * Hkv) * D, dtype=dtype, seed=i) for i in range(L)]
+    kc, vc = (torch.full((L, B, Hkv, slots, D), 3, dtype=torch.uint8 if fp8 else dtype, device=DEV) for _ in "kv")
+    ks, vs = (torch.full((L, B, Hkv, 32), 2.0, device=DEV) if fp8 else None for _ in "kv")
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))] * B))
+    count, path, after = ops.tree_accept(tree, tokens, choice, rows, kc, vc, _i32(lens), ks, vs)
+    want = [6, 6, 5, 1, 0, 0, 6]
+    assert count.tolist() == want
+    assert path.tolist() == [list(range(n)) + [-1] * (N - n) for n in want]
+    assert after.tolist() == [77, 77, 5, 1, -1, -1, 77]
+    for b, n in enumerate(want):
+        at = max(lens[b], 0)
+        for layer in range(L):
+            x = rows[layer].view(B, N, -1, D)[b, :n].transpose(0, 1)
+            for c, sc, new, key in ((kc, ks, x[Hq:Hq + Hkv], True), (vc, vs, x[Hq + Hkv:], False)):
+                whole = torch.full((Hkv, slots, D), 3, dtype=c.dtype, device=DEV)
+                if n:
+                    if fp8:
+                        new, s = ops.kv_quantize_rows(new.cpu(), key)  # torch divides by a reciprocal on the GPU
+                        assert torch.equal(sc[layer, b, :, at:at + n].cpu(), s) and (sc[layer, b, :, at + n:] == 2).all()
+                    whole[:, at:at + n] = new
+                assert torch.equal(c[layer, b], whole)
