@@ -477,11 +477,13 @@ class CausalLM(nn.Module):
     def verify(self, tokens, tree, kv_len, kv_start, cache):
         """One forward over drafted tokens [B, N] (``ops.draft_tree`` with pos0 = kv_len - kv_start): every node of a row is a row of its own that
         sees the row's cache and its ancestors. Returns (final hidden [B*N, H], the layers' rotated [q | k | v] rows, from which
-        ``ops.tree_accept`` appends the accepted nodes to the cache)."""
+        ``ops.tree_accept`` appends the accepted nodes to the cache). Nodes past the model's last position are taken out of ``tree``
+        (their ``see`` becomes 0), so that a path ends before them."""
         cfg = self.cfg
         kv8 = getattr(cache, "fp8", False)
         cos, sin = self.rope(tokens.device)
-        # what is no node may hold any token (an idle row's next one is -1), and a tree may reach past the positions that there are
+        tree.see.masked_fill_(tree.pos >= cfg.max_position, 0)
+        # what is no node may hold any token (an idle row's next one is -1) and any position
         pos = tree.pos.reshape(-1).clamp(0, cfg.max_position - 1)
         x = self.embed_tokens(torch.where(tree.see != 0, tokens, 0).reshape(-1), pos)
         residual, drafts = None, []

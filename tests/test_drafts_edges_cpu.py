@@ -75,3 +75,27 @@ def test_steps_stop_at_the_end_of_the_cache():
         kv_len = kv_len + count
         counts.append((int(count), int(after)))
     assert counts == [(4, 0), (3, 3), (0, -1), (0, -1)] and int(kv_len) == slots
+
+
+@pytest.mark.parametrize("preset", ["tiny-mistral", "tiny-opt"])
+def test_verify_takes_nodes_past_the_last_position_out_of_the_tree(preset):
+    """a cache with more slots than the model has positions: a path ends at the last of them, as if no node had been drafted behind it"""
+    cfg = models.resolve_preset(preset)
+    m = models.CausalLM(cfg, dtype=torch.float32, seed=3)
+    P, N = cfg.max_position, 6
+    lens, starts = [P + 1, P + 1, P + 1, 9], [4, 0, 7, 0]  # node 0 at P - 3, P + 1, P - 6 and 9
+    B = len(lens)
+    cache = KVCache(cfg.num_layers, B, cfg.num_kv_heads, P + 20, cfg.head_dim, "cpu", torch.float32)
+    cache.k.normal_(), cache.v.normal_()
+    tokens = torch.arange(3, 3 + B * N).view(B, N)
+    choice = torch.cat([tokens[:, 1:], tokens[:, :1] + 77], 1)
+    kv_len, start = _i32(lens), _i32(starts)
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))] * B), pos0=kv_len - start)
+    k0 = cache.k.clone()
+    h, drafts = m.verify(tokens, tree, kv_len, start, cache)
+    count, path, after = ops.tree_accept(tree, tokens, choice, drafts, cache.k, cache.v, kv_len)
+    fit = [3, 0, 6, 6]
+    assert count.tolist() == fit
+    assert after.tolist() == [int(choice[b, n - 1]) if n else -1 for b, n in enumerate(fit)]
+    for b, n in enumerate(fit):
+        assert torch.equal(cache.k[:, b, :, lens[b] + n:], k0[:, b, :, lens[b] + n:])
