@@ -81,6 +81,10 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   int lo = a.kv_start ? max(a.kv_start[b], 0) : 0;
   if (a.window) lo = max(lo, len + depth - a.window + 1);
   const int ctx = max(len - lo, 0), n = ctx + a.N;
+  uint64_t near = mine;  // nodes less than `window` places before this one; a place is how many nodes one sees
+  if (a.window && depth + 1 >= a.window)
+    for (int j = 0; j < a.N; ++j)
+      if (depth + 1 - (int)__popcll((uint64_t)see[j]) >= a.window) near &= ~(1ull << j);
   const T* const kc = (const T*)a.kc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   const T* const vc = (const T*)a.vc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   for (int c = tid; c < a.D; c += 256) {
@@ -92,10 +96,7 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   for (int j0 = 0; j0 < n; j0 += 256) {
     const int j = j0 + tid;
     bool sees = j < ctx;
-    if (j >= ctx && j < n) {
-      const int node = j - ctx;
-      sees = (mine >> node & 1) && !(a.window && depth + 1 - __popcll((uint64_t)see[node]) >= a.window);
-    }
+    if (j >= ctx && j < n) sees = near >> (j - ctx) & 1;
     float s = -INFINITY;
     if (sees) {
       const T* kp = j < ctx ? kc + (long)(lo + j) * a.D : x + (long)(j - ctx) * a.ldq + (long)(a.Hq + gh) * a.D;
@@ -176,11 +177,14 @@ __device__ __forceinline__ float* part_of(const TreeArgs& a, int D, int s, long 
 // r / G for a row r of a key head (under 64 G, G up to 4096: the error of the product is under 64 2^-23, and 1 / 2 G is more)
 __device__ __forceinline__ int node_of_row(const TreeArgs& a, int r) { return (int)((r + 0.5f) * a.per_G); }
 
-// ancestors less than `window` positions before a node: the last ones
-__device__ __forceinline__ uint64_t near_nodes(uint64_t see, int window) {
-  if (window)
-    for (int far = __popcll(see) - window; far > 0; --far) see &= see - 1;
-  return see;
+// of the nodes in w, those less than `window` places before the node that sees w; a place is how many nodes one sees (see: the word of this lane's
+// node), so one that sees fewer than `window` has none farther. Every lane of a wave has to be there.
+__device__ __forceinline__ uint64_t near_nodes(uint64_t w, uint64_t see, int window) {
+  const int place = __popcll(w), other = __popcll(see);
+  if (window && __any(place >= window))
+    for (int j = 0; j < NODES; ++j)
+      if (place - __builtin_amdgcn_readlane(other, j) >= window) w &= ~(1ull << j);
+  return w;
 }
 
 // the row that has q longer ones before it (64 rows at most, one a lane)
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
       from[u] = a.window ? ct.len + __popcll(w) - a.window : 0;
       // by the nodes' stage: its first `joint` keys are the context's last ones
       const uint64_t ctx = ~0ull << min(max(from[u] - (ct.len - joint), 0), 63) & ((1ull << joint) - 1);  // joint is 63 at most
-      sees[u] = near_nodes(w, a.window) << joint | ctx;
+      sees[u] = near_nodes(w, see, a.window) << joint | ctx;
     }
     f32x4 o[RT][DT];
     float m[RT], l[RT];

@@ -77,7 +77,8 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                    v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of drafted tokens -> [rows * nodes, Hq * D]. ``qkv`` [rows * nodes, >= (Hq + 2 Hkv) * D] holds the nodes' rotated rows [q | k | v];
     node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
-    key; with ``window`` only those less than ``window`` positions before it. Nothing is appended to the caches; rows that are not
+    key; with ``window`` only those less than ``window`` positions before it (a node's, in masks of the caller's own too, is how many nodes it
+    sees). Nothing is appended to the caches; rows that are not
     nodes come out as zeros. ``out`` may be columns of wider rows, but shares nothing with ``qkv``. What a node does not see, of other
     nodes or outside its window, does not reach it, NaN and infinities among it. uint8 caches hold e4m3 (heads of 128), as
     ``kv_quantize_rows`` and decoding write them, with their slots' scales in ``k_scale``, ``v_scale`` [rows, Hkv, >= Smax]."""

@@ -99,3 +99,16 @@ def test_verify_takes_nodes_past_the_last_position_out_of_the_tree(preset):
     assert after.tolist() == [int(choice[b, n - 1]) if n else -1 for b, n in enumerate(fit)]
     for b, n in enumerate(fit):
         assert torch.equal(cache.k[:, b, :, lens[b] + n:], k0[:, b, :, lens[b] + n:])
+
+
+def test_windows_over_other_masks_than_ancestors():
+    """a node's place is the number of nodes that it sees: those `window` places before it are not seen, wherever their bits are"""
+    see = [1, 2, 0b111, 0b10011, 0b11111]
+    tree = ops.DraftTree(_i32([[-1] * 5]), torch.tensor([see]), _i32([[0] * 5]))
+    qkv, none = torch.randn(5, 12, dtype=torch.float64), torch.zeros(1, 1, 3, 4, dtype=torch.float64)
+    for window in range(1, 7):
+        o = ops.tree_attention(qkv, none, none, _i32([0]), tree, 1, window=window)
+        for i, w in enumerate(see):
+            near = [j for j in range(5) if w >> j & 1 and bin(w).count("1") - bin(see[j]).count("1") < window]
+            p = torch.softmax(qkv[near, 4:8] @ qkv[i, :4] / 2, 0)
+            assert torch.allclose(o[i], p @ qkv[near, 8:], rtol=1e-12, atol=1e-13)

@@ -161,3 +161,18 @@ def test_verify_takes_nodes_past_the_last_position_out_of_the_tree(preset):
     assert after.tolist() == [int(choice[b, n - 1]) if n else -1 for b, n in enumerate(fit)]
     for b, n in enumerate(fit):
         assert torch.equal(cache.k[:, b, :, lens[b] + n:], k0[:, b, :, lens[b] + n:])
+
+
+# ------------------------------------------------------------------------------------------ masks of a caller's own
+@pytest.mark.parametrize("window", [1, 2, 3, 9, 40])
+@pytest.mark.parametrize("Hq,Hkv,D,dtype,fp8", FORMS)
+def test_windows_over_other_masks_than_ancestors(Hq, Hkv, D, dtype, fp8, window):
+    """a node's place is the number of nodes that it sees: those `window` places before it are not seen, wherever their bits are"""
+    g = torch.Generator().manual_seed(window)
+    N = 14
+    see = [[1, 2, 0b111, 0b1111, 0, 0b101101]] * 2
+    for row in range(2):
+        r = torch.rand(N, N, generator=g) < 0.6
+        see[row] = see[row] + [sum(1 << j for j in range(i) if r[i, j]) | 1 << i for i in range(6, N)]
+    _check_masks(see, [50, 0], Hq, Hkv, D, window, 60, dtype, fp8)
+    _check_masks(see, [1900, 70], Hq, Hkv, D, window, 2000, dtype, fp8)
