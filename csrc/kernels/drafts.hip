@@ -61,6 +61,9 @@ struct TreeArgs {
   float* part; int S;                   // partials of at most S shares of a row's keys (part_of)
 };
 
+// the nodes that node i of row b sees; bits past the tree count for nothing
+__device__ __forceinline__ uint64_t word(const TreeArgs& a, int b, int i) { return (uint64_t)a.see[(long)b * a.N + i] & ~0ull >> (NODES - a.N); }
+
 template <typename T>
 __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   extern __shared__ float sm[];  // q [D], acc [D], p [256], sbuf [4]
@@ -69,8 +72,7 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   float* ps = acc + a.D;
   float* sbuf = ps + 256;
   const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, gh = h / (a.Hq / a.Hkv);
-  const int64_t* see = a.see + (long)b * a.N;
-  const uint64_t mine = see[i];
+  const uint64_t mine = word(a, b, i);
   const T* const x = (const T*)a.qkv + (long)b * a.N * a.ldq;
   T* const o = (T*)a.o + ((long)b * a.N + i) * a.ldo + (long)h * a.D;
   if (!mine) {
@@ -84,7 +86,7 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   uint64_t near = mine;  // nodes less than `window` places before this one; a place is how many nodes one sees
   if (a.window && depth + 1 >= a.window)
     for (int j = 0; j < a.N; ++j)
-      if (depth + 1 - (int)__popcll((uint64_t)see[j]) >= a.window) near &= ~(1ull << j);
+      if (depth + 1 - (int)__popcll(word(a, b, j)) >= a.window) near &= ~(1ull << j);
   const T* const kc = (const T*)a.kc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   const T* const vc = (const T*)a.vc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   for (int c = tid; c < a.D; c += 256) {
@@ -146,10 +148,13 @@ __host__ __device__ inline int stages_per_part(int stages, int most, float part_
   return parts > 1 && per + part_cost * parts + join_cost < stages ? per : stages;
 }
 
-// nodes of a row (those that see nothing lie behind them, or between them in plans of a caller's own); every lane of a wave has to be there
+// nodes of a row (those that see nothing lie behind them, or between them in plans of a caller's own, whose masks may name rows behind the last
+// node too); every lane of a wave has to be there
 __device__ __forceinline__ int count_nodes(uint64_t see) {
   const uint64_t live = __ballot(see != 0);
-  return live ? 64 - __builtin_clzll(live) : 0;
+  int n = live ? 64 - __builtin_clzll(live) : 0;
+  while (__any(n < NODES && see >> n)) ++n;
+  return n;
 }
 
 // full: stages that the context fills; rest: its last keys, which go into the nodes' stage where both fit there (and are of one type)
@@ -259,7 +264,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
   }
   if (a.sorted) b = longest(a, b, lane);
   const int G = a.G;
-  const uint64_t see = lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0;
+  const uint64_t see = lane < a.N ? word(a, b, lane) : 0;
   const int n = count_nodes(see), M = n * G;
   const Cut ct = cut(a, b, n, SK);
   if (s >= ct.parts) return;
@@ -750,7 +755,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
   float m = -INFINITY, l = 0.f;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
   int parts = a.S;
-  const int n = count_nodes(lane < a.N ? (uint64_t)a.see[(long)b * a.N + lane] : 0);
+  const int n = count_nodes(lane < a.N ? word(a, b, lane) : 0);
   for (int s0 = 8 * w; s0 < parts; s0 += 8 * WAVES) {
     float2 ml[8];
     f32x4 po[8];
@@ -800,7 +805,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
     }
   }
   if (id >= all || parts == 1 || r >= a.N * G) return;
-  const bool node = a.see[(long)b * a.N + r / G] != 0;  // others have no parts
+  const bool node = word(a, b, r / G) != 0;  // others have no parts
   const float inv = 1.f / l;
   *(uint2*)((bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 16 * c + 4 * g) =
       node ? make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)) : make_uint2(0, 0);

@@ -176,3 +176,14 @@ def test_windows_over_other_masks_than_ancestors(Hq, Hkv, D, dtype, fp8, window)
         see[row] = see[row] + [sum(1 << j for j in range(i) if r[i, j]) | 1 << i for i in range(6, N)]
     _check_masks(see, [50, 0], Hq, Hkv, D, window, 60, dtype, fp8)
     _check_masks(see, [1900, 70], Hq, Hkv, D, window, 2000, dtype, fp8)
+
+
+@pytest.mark.parametrize("window", [0, 4])
+@pytest.mark.parametrize("Hq,Hkv,D,dtype,fp8", FORMS)
+def test_masks_with_bits_of_rows_that_are_no_nodes(Hq, Hkv, D, dtype, fp8, window):
+    """a row behind the last node counts where a mask names it; bits past the tree count for nothing"""
+    past = 1 << 30 | 1 << 63
+    see = [[1 | past, 0b11 | 1 << 9, 0, 0b1011 | 1 << 11, past] + [0] * 7, [0b1 | 1 << 11] + [0] * 11]
+    for lens, slots in (([40, 3], 60), ([1900, 300], 2000)):
+        got = _check_masks(see, lens, Hq, Hkv, D, window, slots, dtype, fp8)
+        assert (got.view(2, 12, -1)[0, 4] == 0).all()
