@@ -75,10 +75,6 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   const uint64_t mine = word(a, b, i);
   const T* const x = (const T*)a.qkv + (long)b * a.N * a.ldq;
   T* const o = (T*)a.o + ((long)b * a.N + i) * a.ldo + (long)h * a.D;
-  if (!mine) {
-    for (int c = tid; c < a.D; c += 256) st(o + c, 0.f);
-    return;
-  }
   const int depth = __popcll(mine) - 1, len = min(max(a.kv_len[b], 0), a.Smax);
   int lo = a.kv_start ? max(a.kv_start[b], 0) : 0;
   if (a.window) lo = max(lo, len + depth - a.window + 1);
@@ -87,6 +83,10 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
   if (a.window && depth + 1 >= a.window)
     for (int j = 0; j < a.N; ++j)
       if (depth + 1 - (int)__popcll(word(a, b, j)) >= a.window) near &= ~(1ull << j);
+  if (!near && (!mine || !ctx)) {  // no node, or one that a window leaves nothing of
+    for (int c = tid; c < a.D; c += 256) st(o + c, 0.f);
+    return;
+  }
   const T* const kc = (const T*)a.kc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   const T* const vc = (const T*)a.vc + ((long)b * a.Hkv + gh) * a.Smax * a.D;
   for (int c = tid; c < a.D; c += 256) {
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void tree_any_kernel(TreeArgs a) {
     }
     __syncthreads();
   }
-  for (int c = tid; c < a.D; c += 256) st(o + c, acc[c] / l);  // a node sees itself
+  for (int c = tid; c < a.D; c += 256) st(o + c, acc[c] / l);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
     bf16x8 qf[RT][DS];
     uint64_t sees[RT];
     int from[RT];  // first key of the context that the row sees
-    bool is_node[RT];
+    bool sees_any[RT];
     const int joint = !KV8 && ct.tiles == ct.full + 1 ? ct.rest : 0;
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
@@ -286,11 +286,12 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
 #pragma unroll
       for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
       const uint64_t w = lane64(see, node);
-      is_node[u] = w != 0;
       from[u] = a.window ? ct.len + __popcll(w) - a.window : 0;
       // by the nodes' stage: its first `joint` keys are the context's last ones
       const uint64_t ctx = ~0ull << min(max(from[u] - (ct.len - joint), 0), 63) & ((1ull << joint) - 1);  // joint is 63 at most
-      sees[u] = near_nodes(w, see, a.window) << joint | ctx;
+      const uint64_t near = near_nodes(w, see, a.window);
+      sees[u] = near << joint | ctx;
+      sees_any[u] = near || (w && max(from[u], ct.lo) < ct.len);
     }
     f32x4 o[RT][DT];
     float m[RT], l[RT];
@@ -722,12 +723,12 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
 #pragma unroll
         for (int c = 0; c < DT; ++c) q[64 * c] = o[u][c];
       } else if (r < M) {
-        const float inv = 1.f / l[u];  // a node sees itself
+        const float inv = 1.f / l[u];
         const int node = node_of_row(a, r);
         bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + node) * a.ldo + (long)(gh * G + r - node * G) * D + 4 * g;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
-          *(uint2*)(p + 16 * c) = is_node[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
+          *(uint2*)(p + 16 * c) = sees_any[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
                                           : make_uint2(0, 0);
       }
     }
@@ -805,7 +806,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(TreeArgs a, int SK) {
     }
   }
   if (id >= all || parts == 1 || r >= a.N * G) return;
-  const bool node = word(a, b, r / G) != 0;  // others have no parts
+  const bool node = word(a, b, r / G) != 0;  // others have no parts (windows that may leave nothing of a node are under a stage: never cut)
   const float inv = 1.f / l;
   *(uint2*)((bf16_t*)a.o + ((long)b * a.N + r / G) * a.ldo + (long)(gh * G + r % G) * D + 16 * c + 4 * g) =
       node ? make_uint2(pack2bf(o[0] * inv, o[1] * inv), pack2bf(o[2] * inv, o[3] * inv)) : make_uint2(0, 0);

@@ -187,3 +187,13 @@ def test_masks_with_bits_of_rows_that_are_no_nodes(Hq, Hkv, D, dtype, fp8, windo
     for lens, slots in (([40, 3], 60), ([1900, 300], 2000)):
         got = _check_masks(see, lens, Hq, Hkv, D, window, slots, dtype, fp8)
         assert (got.view(2, 12, -1)[0, 4] == 0).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,dtype,fp8", FORMS)
+def test_masks_that_leave_nothing_of_a_node(Hq, Hkv, D, dtype, fp8):
+    """a window that holds none of a node's keys: zeros, beside nodes that see some"""
+    see = [[1, 2, 4, 0b111, 0b11111, 0b100001]]  # node 3 sees three nodes at places 1, two or more before its own
+    for window in (1, 2):
+        for n, slots in ((0, 60), (50, 60), (1900, 2000)):
+            got = _check_masks(see, [n], Hq, Hkv, D, window, slots, dtype, fp8)
+            assert (got[3] == 0).all()
