@@ -49,22 +49,31 @@ void whole(const Tensor& t, at::ScalarType type, at::IntArrayRef shape, const Te
                     t.scalar_type(), " ", t.sizes());
 }
 
-// rows that share no element: other memory, or other columns of the same rows
-bool apart(const Tensor& a, const Tensor& b) {
-  if (!a.numel() || !b.numel() || !a.is_alias_of(b)) return true;
-  const int64_t size = a.element_size(), la = (a.size(0) - 1) * a.stride(0) + a.size(1), lb = (b.size(0) - 1) * b.stride(0) + b.size(1);
-  const char *pa = (const char*)a.data_ptr(), *pb = (const char*)b.data_ptr();
-  if (pa + la * size <= pb || pb + lb * size <= pa) return true;
-  const int64_t pitch = b.stride(0), bytes = pa - pb;
-  if (a.stride(0) != pitch || pitch == 0 || bytes % size) return false;
-  const int64_t col = ((bytes / size) % pitch + pitch) % pitch;  // a's first column, of b's
-  return col >= b.size(1) && col + a.size(1) <= pitch;
+// memory of `rows` pieces of `width` bytes, `pitch` apart
+struct Span { const char* at; int64_t rows, pitch, width; };
+Span span(const Tensor& t) {  // contiguous behind its first dimension, or all of it
+  const int64_t size = t.element_size();
+  if (!t.numel() || t.is_contiguous()) return {(const char*)t.data_ptr(), 1, 0, t.numel() * size};
+  return {(const char*)t.data_ptr(), t.size(0), t.stride(0) * size, t.numel() / t.size(0) * size};
 }
-
-bool shares(const Tensor& a, const Tensor& b) {
-  const auto s = at::get_overlap_status(a, b);
-  return s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial;
+// a piece that lies in none of the rows of b
+bool apart(const char* from, const char* to, const Span& b) {
+  if (b.rows == 1 || b.pitch <= 0) return to <= b.at || b.at + b.width <= from;
+  const int64_t first = from < b.at + b.width ? 0 : (from - b.at - b.width) / b.pitch + 1;  // the first row that ends behind `from`
+  return first >= b.rows || to <= b.at + first * b.pitch;
 }
+// two that share no byte: other memory, or other columns of the same rows
+bool apart(const Span& a, const Span& b) {
+  if (!a.width || !b.width) return true;
+  if (a.rows == 1) return apart(a.at, a.at + a.width, b);
+  if (b.rows == 1) return apart(b.at, b.at + b.width, a);
+  if (a.at + (a.rows - 1) * a.pitch + a.width <= b.at || b.at + (b.rows - 1) * b.pitch + b.width <= a.at) return true;
+  if (a.pitch != b.pitch || a.pitch <= 0) return false;
+  const int64_t col = ((a.at - b.at) % a.pitch + a.pitch) % a.pitch;  // a's first column, of b's
+  return col >= b.width && col + a.width <= a.pitch;
+}
+// layers that are written at once: each has memory of its own
+bool layers_apart(const Tensor& t) { return t.size(0) <= 1 || !t.numel() || t.stride(0) >= t[0].numel(); }
 
 // the slots' scales of an e4m3 cache [.., rows, heads, slots, 128], alike for keys and values
 struct Scales { float* k = nullptr; float* v = nullptr; long layer = 0; int slots = 0; };
@@ -141,7 +150,10 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   TORCH_CHECK_VALUE(out.scalar_type() == qkv.scalar_type() && out.dim() == 2 && out.size(0) == B * N && out.size(1) == Hq * D &&
                         (out.stride(1) == 1 || out.size(0) == 0), "tree_attention: out shape");
   at::assert_no_internal_overlap(out);
-  TORCH_CHECK_VALUE(apart(out, qkv) && !shares(out, kc) && !shares(out, vc), "tree_attention: out overlaps what is read");
+  const Span to = span(out);
+  TORCH_CHECK_VALUE(apart(to, span(qkv)) && apart(to, span(kc)) && apart(to, span(vc)) && apart(to, span(see)) && apart(to, span(kv_len)) &&
+                        (!has(kv_start) || apart(to, span(*kv_start))) && (!sc.k || (apart(to, span(*k_scale)) && apart(to, span(*v_scale)))),
+                    "tree_attention: out overlaps what is read");
   const int64_t S = qkv.scalar_type() == at::kBFloat16 && al(kc, 16) && al(vc, 16)
                         ? rt_tree_parts((int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window) : 0;
   TORCH_CHECK_VALUE(S || !sc.k || !B, "tree_attention: an e4m3 cache of this size");
@@ -170,8 +182,9 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
   TORCH_CHECK_VALUE(D > 0 && Hkv > 0, "tree_accept: caches of no heads");
   TORCH_CHECK_VALUE(vc.scalar_type() == kc.scalar_type() && vc.sizes() == kc.sizes() && vc.strides() == kc.strides() && kc[0].is_contiguous(),
               "tree_accept: caches of one type and layout, contiguous in each layer");
-  TORCH_CHECK_VALUE(!shares(kc, vc), "tree_accept: keys and values of one memory");
   const Scales sc = scales(kc, k_scale, v_scale);
+  TORCH_CHECK_VALUE(layers_apart(kc) && (!sc.k || layers_apart(*k_scale)), "tree_accept: layers of one memory");
+  TORCH_CHECK_VALUE(apart(span(kc), span(vc)) && (!sc.k || apart(span(*k_scale), span(*v_scale))), "tree_accept: keys and values of one memory");
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
   whole(see, at::kLong, {B, N}, kc, "tree_accept tree");
@@ -182,6 +195,7 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
     TORCH_CHECK_VALUE(x.scalar_type() == (sc.k ? at::kBFloat16 : kc.scalar_type()) && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
                     x.stride(0) == drafts[0].stride(0) && x.size(0) == B * N,
                 "tree_accept: drafts [rows nodes, (heads + 2 key heads) dim] of the caches' type, alike in every layer");
+    TORCH_CHECK_VALUE(apart(span(x), span(kc)) && apart(span(x), span(vc)), "tree_accept: drafts in the caches' memory");
     copy = copy || (sc.k && (!al(x, 16) || x.stride(0) % 8));
   }
   // keys lie behind `heads` queries; where nobody said how many (0), the rows hold nothing behind [q | k | v]

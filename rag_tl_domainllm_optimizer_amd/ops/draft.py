@@ -138,6 +138,10 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
         raise ValueError("tokens and choice: int64 expected")
     if D < 1 or Hkv < 1:
         raise ValueError("caches of no heads")
+    for a, b in ((k_cache, v_cache), (k_scale, v_scale)):
+        if a is not None and b is not None and a.numel() and (a.data_ptr() == b.data_ptr() or any(
+                st == 0 and n > 1 for t in (a, b) for st, n in zip(t.stride(), t.shape))):
+            raise ValueError("layers, or keys and values, of one memory")
     fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
     if len(drafts) != L or any(x.dim() != 2 or x.shape != drafts[0].shape or (x.dtype != k_cache.dtype and not fp8) or x.shape[0] != B * tree.shape[1]
                                for x in drafts):

@@ -112,3 +112,22 @@ def test_windows_over_other_masks_than_ancestors():
             near = [j for j in range(5) if w >> j & 1 and bin(w).count("1") - bin(see[j]).count("1") < window]
             p = torch.softmax(qkv[near, 4:8] @ qkv[i, :4] / 2, 0)
             assert torch.allclose(o[i], p @ qkv[near, 8:], rtol=1e-12, atol=1e-13)
+
+
+# ------------------------------------------------------------------------------------------ memory that is shared
+def _store(kc, vc, ks=None, vs=None):
+    L, B, Hkv, _, D = kc.shape
+    return ops.tree_accept(ops.draft_tree(_i32([[-1, 0]] * B)), *(torch.zeros(B, 2, dtype=torch.int64) for _ in "tc"), [torch.zeros(2 * B, 3 * Hkv * D)] * L,
+                           kc, vc, _i32([3] * B), ks, vs)
+
+
+@pytest.mark.parametrize("bad", [
+    lambda: _store(torch.zeros(1, 1, 1, 9, 4).expand(2, 1, 1, 9, 4), torch.zeros(2, 1, 1, 9, 4)),
+    lambda: _store(torch.zeros(2, 1, 1, 9, 4), torch.zeros(2, 1, 1, 9, 4)[:, :, :1].expand(2, 1, 3, 9, 4)),
+    lambda: _store(*[torch.zeros(2, 1, 1, 9, 4)] * 2),
+    lambda: _store(*(torch.zeros(2, 1, 1, 9, 128, dtype=torch.uint8) for _ in "kv"), torch.ones(1, 1, 1, 9).expand(2, 1, 1, 9), torch.ones(2, 1, 1, 9)),
+    lambda: _store(*(torch.zeros(2, 1, 1, 9, 128, dtype=torch.uint8) for _ in "kv"), *[torch.ones(2, 1, 1, 9)] * 2),
+])
+def test_accept_refuses_layers_of_one_memory(bad):
+    with pytest.raises(ValueError):
+        bad()

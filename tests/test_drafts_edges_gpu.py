@@ -197,3 +197,69 @@ def test_masks_that_leave_nothing_of_a_node(Hq, Hkv, D, dtype, fp8):
         for n, slots in ((0, 60), (50, 60), (1900, 2000)):
             got = _check_masks(see, [n], Hq, Hkv, D, window, slots, dtype, fp8)
             assert (got[3] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------ memory that is shared
+def _store(kc, vc, ks=None, vs=None, drafts=None):
+    L, B, Hkv, _, D = kc.shape
+    return ops.tree_accept(ops.draft_tree(_i32([[-1, 0]] * B)), *(torch.zeros(B, 2, dtype=torch.int64, device=DEV) for _ in "tc"),
+                           [_rand(2 * B, 3 * Hkv * D)] * L if drafts is None else drafts, kc, vc, _i32([3] * B), ks, vs)
+
+
+def _bytes(*shape):
+    return torch.zeros(*shape, dtype=torch.uint8, device=DEV)
+
+
+def _ones(*shape):
+    return torch.ones(*shape, device=DEV)
+
+
+@pytest.mark.parametrize("bad", [
+    lambda: _store(*(_rand(1, 1, 1, 9, 64).expand(2, 1, 1, 9, 64) for _ in "kv")),
+    lambda: _store(*(_rand(2 * 9 * 64).as_strided((2, 1, 1, 9, 64), (8 * 64, 9 * 64, 9 * 64, 64, 1)) for _ in "kv")),
+    lambda: _store(*[_rand(2, 3, 1, 9, 64)[:, :2]] * 2),                               # parts of one larger cache
+    lambda: _store(*(lambda c: (c[:, :2], c[:, 1:]))(_rand(2, 3, 1, 9, 64))),
+    lambda: _store(*(_bytes(2, 1, 1, 9, 128) for _ in "kv"), *(_ones(1, 1, 1, 9).expand(2, 1, 1, 9) for _ in "kv")),
+    lambda: _store(*(_bytes(2, 1, 1, 9, 128) for _ in "kv"), *[_ones(2, 1, 1, 9)] * 2),
+    lambda: _store(*(_bytes(2, 2, 1, 9, 128)[:, :1] for _ in "kv"), *[_ones(2, 2, 1, 9)[:, :1]] * 2),
+    lambda: (lambda c: _store(c, c.clone(), drafts=[c.view(-1)[:2 * 192].view(2, 192)]))(_rand(1, 1, 1, 9, 64)),
+    lambda: (lambda c: _store(c.clone(), c, drafts=[c.view(-1)[64:].as_strided((2, 192), (200, 1))]))(_rand(1, 1, 1, 9, 64)),
+])
+def test_accept_refuses_memory_that_is_shared(bad):
+    with pytest.raises(ValueError):
+        bad()
+
+
+def _attend_into(out, qkv=None, kc=None, vc=None):
+    return ops.tree_attention(_rand(2, 512) if qkv is None else qkv, _rand(1, 2, 9, 64) if kc is None else kc, _rand(1, 2, 9, 64) if vc is None else vc, _i32([3]),
+                              ops.draft_tree(_i32([[-1, 0]])), 4, out=out)
+
+
+@pytest.mark.parametrize("at", [-300, -255, 0, 100, 1151, 1200])
+def test_attention_refuses_an_output_that_is_in_the_cache(at):
+    """columns of wider rows: some of them, or the space between them, hold the cache"""
+    store = torch.zeros(8000, dtype=BF16, device=DEV)
+    cache = store[2000:2000 + 1152].view(1, 2, 9, 64)
+    for pitch in (256, 300, 700):  # two rows of 256 columns
+        out = store.as_strided((2, 256), (pitch, 1), 2000 + at)
+        rows = [(2000 + at + i * pitch, 2000 + at + i * pitch + 256) for i in range(2)]
+        free = all(b <= 2000 or a >= 3152 for a, b in rows)
+        for which in ("kc", "vc"):
+            if free:
+                _attend_into(out, **{which: cache})
+            else:
+                with pytest.raises(ValueError):
+                    _attend_into(out, **{which: cache})
+
+
+def test_attention_beside_a_cache_in_one_allocation():
+    """output, rows and caches as parts of one allocation"""
+    store = _rand(20000, seed=1)
+    kc, vc = store[:1152].view(1, 2, 9, 64), store[1152:2304].view(1, 2, 9, 64)
+    wide = store[2304:2304 + 2 * 800].view(2, 800)
+    want = ops.tree_attention(wide[:, :512].clone(), kc.clone(), vc.clone(), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4)
+    assert torch.equal(_attend_into(wide[:, 512:768], wide[:, :512], kc, vc), want)
+    around = store[4000:4000 + 2 * 3000].view(2, 3000)  # rows with the cache in the space between them
+    cache = around[0, 304:304 + 1152].view(1, 2, 9, 64)  # at 16 bytes, as the other one: the same form
+    cache.copy_(kc)
+    assert torch.equal(_attend_into(around[:, :256], store[12000:12000 + 1024].view(2, 512).copy_(wide[:, :512]), cache, vc), want)
