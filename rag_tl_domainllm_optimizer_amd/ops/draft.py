@@ -103,6 +103,8 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"window {window}, scale {scale}")
     if torch.is_grad_enabled() and any(t.requires_grad for t in (qkv, k_cache, v_cache)):
         raise ValueError("tree_attention has no gradient")
+    if out is not None and (out.dtype != qkv.dtype or tuple(out.shape) != (B * N, Hq * D)):
+        raise ValueError(f"out: {qkv.dtype} {(B * N, Hq * D)} expected, got {out.dtype} {tuple(out.shape)}")
     kv_len = _ints(kv_len, "kv_len", (B,), qkv)
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
     if fp8:

@@ -131,3 +131,12 @@ def _store(kc, vc, ks=None, vs=None):
 def test_accept_refuses_layers_of_one_memory(bad):
     with pytest.raises(ValueError):
         bad()
+
+
+@pytest.mark.parametrize("out", [torch.zeros(6, 4), torch.zeros(3, 2, 4), torch.zeros(2, 4, dtype=torch.float64), torch.zeros(2, 5), torch.zeros(8)])
+def test_attention_refuses_an_output_of_another_shape(out):
+    """one row would be copied into every row of an output with more"""
+    with pytest.raises(ValueError):
+        ops.tree_attention(torch.randn(2, 12), *(torch.randn(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 1, out=out)
+    with pytest.raises(ValueError):
+        ops.tree_attention(torch.randn(1, 12), *(torch.randn(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1]])), 1, out=out)
