@@ -15,7 +15,7 @@ extern "C" {
 int rt_draft_tree(const int*, const int*, const int*, int, int, int64_t*, int*, hipStream_t);
 int rt_tree_parts(int, int, int, int, int, int, int);
 int rt_tree_attention(int, const void*, long, const void*, const void*, const float*, const float*, int, const int*, const int*, const int64_t*,
-                      void*, long, float*, int, int, int, int, int, int, int, int, float, hipStream_t);
+                      void*, long, float*, int, int, int, int, int, int, int, int, float, int, hipStream_t);
 int rt_tree_accept(const int*, const int64_t*, const int64_t*, const int64_t*, const int*, int*, int*, int64_t*, const void* const*, long, void*,
                    void*, long, float*, float*, long, int, int, int, int, int, int, int, int, int, hipStream_t);
 int rt_alternatives(int, const void*, long, const int64_t*, float, long, int, int, float*, float*, float*, int64_t*, float*, hipStream_t);
@@ -123,13 +123,14 @@ std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parent_, const optio
 
 Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& kv_len_, const optional<Tensor>& kv_start_,
                       const Tensor& see, const optional<Tensor>& out_, int64_t Hq, int64_t window, const optional<double>& scale_,
-                      const optional<Tensor>& k_scale, const optional<Tensor>& v_scale) {
+                      const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, bool as_stored) {
   act(qkv, "tree_attention qkv");
   TORCH_CHECK_VALUE(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && (qkv.stride(1) == 1 || qkv.size(0) == 0),
                     "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim] expected, got ", qkv.sizes(), ", ", kc.sizes());
   const int64_t B = kc.size(0), Hkv = kc.size(1), Smax = kc.size(2), D = kc.size(3), N = see.size(1);
   TORCH_CHECK_VALUE(N >= 1 && N <= 64, "tree_attention: 1 to 64 nodes a row expected, got a tree ", see.sizes());
   const Scales sc = scales(kc, k_scale, v_scale);
+  TORCH_CHECK_VALUE(sc.k || !as_stored, "tree_attention: only an e4m3 cache stores nodes otherwise than they are");
   TORCH_CHECK_VALUE(sc.k ? qkv.scalar_type() == at::kBFloat16 : kc.scalar_type() == qkv.scalar_type(), "caches of ", kc.scalar_type(),
                     " under queries of ", qkv.scalar_type());
   whole(kc, kc.scalar_type(), kc.sizes(), qkv, "tree_attention k_cache");
@@ -164,7 +165,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
   Tensor part = S > 1 ? at::empty({S * B * Hkv * ((N * (Hq / Hkv) + 15) / 16) * 16 * (D + 2)}, qkv.options().dtype(at::kFloat)) : Tensor();
   rc_ok(rt_tree_attention(x.scalar_type() == at::kFloat, x.data_ptr(), x.stride(0), kc.data_ptr(), vc.data_ptr(), sc.k, sc.v, sc.slots,
                           kv_len.data_ptr<int>(), ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
-                          (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, stream()), "tree_attention");
+                          (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, as_stored, stream()), "tree_attention");
   if (!o.is_same(out)) out.copy_(o);
   return out;
 }

@@ -240,13 +240,17 @@ __device__ __forceinline__ float fp8_at(uint32_t four, int e) {
   return f[e & 1];
 }
 
+// a value of a row with this scale, as the row is read once it lies in an e4m3 cache
+__device__ __forceinline__ float as_stored(float v, float scale) { return fp8_at(__builtin_amdgcn_cvt_pk_fp8_f32(v * (1.f / scale), 0.f, 0, false), 0) * scale; }
+
 // The bound: 128 registers where two workgroups of eight waves share a CU (in e4m3, with 162: rows of 128 queries 91 us, with the bound 81); elsewhere 256,
 // without which the compiler keeps some in the matrix cores' file and moves them in each stage (32 rows of 5 nodes, 12 heads of 64: 11.3 us, with
 // it 10.7; 64 rows of 64 nodes 209 and 205).
-template <int D, int RT, int WR, int WK, int KT, bool KV8>
+// STORED: the nodes' keys and values count as they will be once they lie in the e4m3 cache.
+template <int D, int RT, int WR, int WK, int KT, bool KV8, bool STORED>
 __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kernel(TreeArgs a) {
   constexpr int NW = WR * WK, SK = WK * KT, ROWS = 16 * RT * WR, KB = SK * D * 2, DS = D / 32, DT = D / 16, KS = KT / 16, NC = D / 8;
-  static_assert(KB / 1024 % NW == 0 && SK >= NODES && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
+  static_assert(KB / 1024 % NW == 0 && SK >= NODES && (KV8 || !STORED) && (!KV8 || (D == 128 && SK == 64 && NW >= 2)));
   __shared__ __attribute__((aligned(128))) char smem[4 * KB];
   __shared__ __attribute__((aligned(16))) float scales[KV8 ? 4 : 1][KV8 ? 2 * SK : 1];  // of a stage's keys, and of its values
   __shared__ unsigned bad[2][2];  // keys of the first stage, and of the nodes', whose values are not all numbers
@@ -402,15 +406,16 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
     // own keys, 3: the context's last keys, repeated behind its end
     auto multiply = [&](auto mode, int t, char* image) {
       constexpr int MODE = decltype(mode)::value;
-      constexpr bool SCALED = KV8 && MODE != 2;
-      char* const Ks = image + wk * KT * D * (SCALED ? 1 : 2);
-      char* const Vs = Ks + (SCALED ? KB / 2 : KB);
+      constexpr bool RAW = KV8 && MODE != 2, SCALED = RAW || STORED;
+      char* const Ks = image + wk * KT * D * (RAW ? 1 : 2);
+      char* const Vs = Ks + (RAW ? KB / 2 : KB);
+      const float* const scale_of = scales[RAW ? t - t0 & 3 : 0];
       f32x4 st[KS][RT];
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int u = 0; u < RT; ++u) st[k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if constexpr (SCALED) {
+      if constexpr (RAW) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -438,7 +443,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
       if constexpr (SCALED) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const f32x4 sc = *(const f32x4*)&scales[t - t0 & 3][key0 + 16 * k];
+          const f32x4 sc = *(const f32x4*)&scale_of[key0 + 16 * k];
 #pragma unroll
           for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -512,11 +517,11 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
       if constexpr (SCALED) {
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const f32x4 sc = *(const f32x4*)&scales[t - t0 & 3][SK + key0 + 16 * k];
+          const f32x4 sc = *(const f32x4*)&scale_of[SK + key0 + 16 * k];
 #pragma unroll
           for (int u = 0; u < RT; ++u)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) st[k][u][e] *= MODE == 0 || (MODE == 1 ? fabsf(sc[e]) < INFINITY : key0 + 16 * k + e < ct.rest) ? sc[e] : 0.f;
+            for (int e = 0; e < 4; ++e) st[k][u][e] *= MODE == 0 || (MODE != 3 ? fabsf(sc[e]) < INFINITY : key0 + 16 * k + e < ct.rest) ? sc[e] : 0.f;
         }
       }
       bf16x8 pf[KT / 32][RT];
@@ -544,7 +549,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
         return v;
       };
       const int key_a = 4 * g + (lane >> 2 & 3), pcol = lane & 3;  // transposed reads: rows 16 apart have the same swizzle
-      if constexpr (SCALED) {
+      if constexpr (RAW) {
         // lane pairs read the 16 columns of keys 4 g .. + 3 and 16 behind these; the lane gets its column of the eight
         const int q = lane >> 1 & 7, key = 4 * g + (q & 3) + 16 * (q >> 2);
         const uint32_t at = lds_addr(Vs + key * D + 16 * v8_chunk(key, 0) + 8 * (lane & 1));
@@ -612,9 +617,26 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
           }
           bool ill = x[0] != w[h][0] || x[1] != w[h][1] || x[2] != w[h][2] || x[3] != w[h][3];
           if (ill) *(u32x4*)(values + e + h * second) = x;
-          if (raw) ill |= !(fabsf(scales[0][SK + key]) < INFINITY);
+          if (raw || STORED) ill |= !(fabsf(scales[0][SK + key]) < INFINITY);
           if (ill) atomicOr(&bad[own.value][key / 32], 1u << (key % 32));
         }
+      }
+    };
+    // The nodes' keys and values to e4m3 and back, with a scale each in the place of a stage that is done: as tree_accept stores them. 16 lanes a row,
+    // each with 8 elements, wherever the swizzle put these.
+    auto round_nodes = [&](char* image) {
+#pragma unroll 1
+      for (int e = 16 * tid; e < 2 * KB; e += 16 * 64 * NW) {
+        float f[8], am = 0.f;
+        unpack8(*(const uint4*)(image + e), f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(f[i]));
+#pragma unroll
+        for (int i = 1; i < 16; i <<= 1) am = fmaxf(am, __shfl_xor(am, i, 16));
+        const float sc = am > 0.f ? am / 448.f : 1.f;
+        const uint2 q = f32x8_to_fp8(f, 1.f / sc);
+        *(bf16x8*)(image + e) = fp8x8_to_bf16(q.x, q.y);
+        if ((tid & 15) == 0) scales[0][e / (2 * D)] = sc;
       }
     };
     auto turn = [&](auto mode, int t) {
@@ -645,6 +667,11 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
       if (MODE != 2 && t + 1 < t1) stage(t + 1, cur ^ 1);
       char* const image = smem + 2 * cur * KB;
       cur ^= 1;
+      if constexpr (MODE == 2 && STORED) {
+        round_nodes(image);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+      }
       if constexpr (MODE == 1 || MODE == 2) {
         only_numbers(image + KB, std::bool_constant<MODE == 2>());
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -674,7 +701,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
               const uint32_t four = KV8 && !own ? *(const uint32_t*)(v8 + 16 * c) : 0;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float f = KV8 && !own ? fp8_at(four, e) * sc : bf2f(v[16 * c + e]);
+                const float f = KV8 && !own ? fp8_at(four, e) * sc : STORED ? as_stored(bf2f(v[16 * c + e]), scales[0][SK + key]) : bf2f(v[16 * c + e]);
                 if (!(fabsf(f) < INFINITY)) o[u][c][e] += f;
               }
               asm volatile("" ::: "memory");  // this is seldom reached: few registers, not many loads at once
@@ -911,23 +938,23 @@ extern "C" int rt_draft_tree(const int* parent, const int* nodes, const int* pos
 
 constexpr int WIDE_ROWS = 192;  // rows of a key head that go to workgroups of 64
 
-template <int D, int RT, int WR, int WK, int KT, bool KV8>
+template <int D, int RT, int WR, int WK, int KT, bool KV8, bool STORED>
 static void launch_tree_form(const TreeArgs& a, int rows, hipStream_t stream) {
   TreeArgs t = a;
   t.blocks = (rows + 16 * RT * WR - 1) / (16 * RT * WR);
   const dim3 grid = t.blocks == 1 ? dim3(a.S, a.Hkv, a.B) : dim3(8 * t.blocks, (unsigned)(((long)a.S * a.B * a.Hkv + 7) / 8));
-  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT, KV8>), grid, dim3(64 * WR * WK), 0, stream, t);
+  hipLaunchKernelGGL((tree_mfma_kernel<D, RT, WR, WK, KT, KV8, STORED>), grid, dim3(64 * WR * WK), 0, stream, t);
 }
-template <int D, bool KV8>
+template <int D, bool KV8, bool STORED>
 static int launch_tree(const TreeArgs& a, int rows, hipStream_t stream) {
   // waves by rows of 16, and two shares of each stage's keys: half the chain of a stage, and the shares are joined in LDS at the end (16 ungrouped
   // rows of 32 nodes 52 -> 47 us, 48 rows of 64 34 -> 31 against one share). Up to 192 rows go to workgroups of 64, two of them on a
   // CU, that read the same keys from L2 (32 rows of 128 over 500 to 2900 keys 56 us, in one workgroup of 8 waves with two tiles each 64); beyond, and
   // with few idle waves, two tiles a wave halve the reads of LDS (40 rows of 240 41 us against 46).
-  if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32, KV8>(a, rows, stream);
-  else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32, KV8>(a, rows, stream);
-  else if (rows <= WIDE_ROWS) launch_tree_form<D, 1, 4, 2, 32, KV8>(a, rows, stream);
-  else launch_tree_form<D, 2, 8, 1, 64, KV8>(a, rows, stream);
+  if (rows <= 16) launch_tree_form<D, 1, 1, 2, 32, KV8, STORED>(a, rows, stream);
+  else if (rows <= 32) launch_tree_form<D, 1, 2, 2, 32, KV8, STORED>(a, rows, stream);
+  else if (rows <= WIDE_ROWS) launch_tree_form<D, 1, 4, 2, 32, KV8, STORED>(a, rows, stream);
+  else launch_tree_form<D, 2, 8, 1, 64, KV8, STORED>(a, rows, stream);
   RT_LAUNCH_CHECK();
   return 0;
 }
@@ -962,10 +989,11 @@ extern "C" int rt_tree_parts(int B, int N, int Hq, int Hkv, int D, int Smax, int
 
 extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void* kc, const void* vc, const float* ksc, const float* vsc, int SmaxP,
                                  const int* kv_len, const int* kv_start, const int64_t* see, void* o, long ldo, float* part, int S, int B, int N, int Hq, int Hkv, int D, int Smax,
-                                 int window, float scale, hipStream_t stream) {
+                                 int window, float scale, int stored, hipStream_t stream) {
   if (B == 0) return 0;
   if (N < 1 || N > NODES || Hkv < 1 || Hq % Hkv || Hq > 65535 || B > 65535 || D < 1 || D > 512) return -1;
   TreeArgs a{qkv, ldq, kc, vc, ksc, vsc, SmaxP, kv_len, kv_start, see, o, ldo, B, N, Hq, Hkv, D, Smax, window, scale, Hq / Hkv, 1.f / (Hq / Hkv), 0, 1, 0.f, 0.f, part, S};
+  if (stored && !ksc) return -1;
   if (ksc && (!vsc || D != 128 || SmaxP < Smax || S < 1)) return -1;
   if (S < 1) {
     const size_t shm = (2 * D + 256 + 4) * sizeof(float);
@@ -981,8 +1009,8 @@ extern "C" int rt_tree_attention(int f32, const void* qkv, long ldq, const void*
   // Long rows first where a CU takes workgroups of 256 rows one after the other: 64 rows of 300 to 4000 keys in any order 177 us, as they come 230.
   // Smaller workgroups, of which several share a CU, only pay for the order (64 rows over 32 ungrouped heads 102 us, in order 110).
   a.sorted = rows > WIDE_ROWS && B > 1 && B <= 64 && (long)B * Hkv * S > num_cus();
-  const int rc = ksc ? launch_tree<128, true>(a, rows, stream) : D == 128 ? launch_tree<128, false>(a, rows, stream)
-                                                                          : launch_tree<64, false>(a, rows, stream);
+  const int rc = ksc ? (stored ? launch_tree<128, true, true>(a, rows, stream) : launch_tree<128, true, false>(a, rows, stream))
+                     : D == 128 ? launch_tree<128, false, false>(a, rows, stream) : launch_tree<64, false, false>(a, rows, stream);
   if (rc) return rc;
   if (S > 1) {
     const long all = (long)B * Hkv * ((rows + 15) / 16) * (D / 16);

@@ -474,11 +474,13 @@ class CausalLM(nn.Module):
         return self.final_norm(x, residual)
 
     @torch.no_grad()
-    def verify(self, tokens, tree, kv_len, kv_start, cache):
+    def verify(self, tokens, tree, kv_len, kv_start, cache, as_stored: bool = False):
         """One forward over drafted tokens [B, N] (``ops.draft_tree`` with pos0 = kv_len - kv_start): every node of a row is a row of its own that
         sees the row's cache and its ancestors. Returns (final hidden [B*N, H], the layers' rotated [q | k | v] rows, from which
         ``ops.tree_accept`` appends the accepted nodes to the cache). Nodes past the model's last position are taken out of ``tree``
-        (their ``see`` becomes 0), so that a path ends before them."""
+        (their ``see`` becomes 0), so that a path ends before them. Over an fp8 cache, nodes attend to each other's keys and values before they are
+        rounded, as a prompt's tokens do; with ``as_stored`` to the rounded ones that :meth:`decode` sees, so that an answer does not depend on
+        how much of it was drafted at once."""
         cfg = self.cfg
         kv8 = getattr(cache, "fp8", False)
         cos, sin = self.rope(tokens.device)
@@ -493,7 +495,8 @@ class CausalLM(nn.Module):
                 qkv = ops.rope_qkv(qkv, pos, cos, sin, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim)
             drafts.append(qkv)
             ks, vs = cache.scales(li) if kv8 else (None, None)
-            o = ops.tree_attention(qkv, cache.k[li], cache.v[li], kv_len, tree, cfg.num_heads, kv_start, cfg.sliding_window, k_scale=ks, v_scale=vs)
+            o = ops.tree_attention(qkv, cache.k[li], cache.v[li], kv_len, tree, cfg.num_heads, kv_start, cfg.sliding_window, k_scale=ks, v_scale=vs,
+                                   as_stored=as_stored and kv8)
             x, residual = layer.mlp(o, residual)
         return self.final_norm(x, residual), drafts
 

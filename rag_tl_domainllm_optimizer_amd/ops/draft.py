@@ -74,16 +74,18 @@ def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0:
 def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len: torch.Tensor, tree: DraftTree, Hq: int,
                    kv_start: Optional[torch.Tensor] = None, window: int = 0, scale: Optional[float] = None,
                    out: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
-                   v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   v_scale: Optional[torch.Tensor] = None, as_stored: bool = False) -> torch.Tensor:
     """Attention of drafted tokens -> [rows * nodes, Hq * D]. ``qkv`` [rows * nodes, >= (Hq + 2 Hkv) * D] holds the nodes' rotated rows [q | k | v];
     node i sees the slots [kv_start, kv_len) of its row in the caches [rows, Hkv, Smax, D] and its ancestors' and its own
     key; with ``window`` only those less than ``window`` positions before it (a node's, in masks of the caller's own too, is how many nodes it
     sees). Nothing is appended to the caches; rows that are not
     nodes come out as zeros. ``out`` may be columns of wider rows, but shares nothing with ``qkv``. What a node does not see, of other
     nodes or outside its window, does not reach it, NaN and infinities among it. uint8 caches hold e4m3 (heads of 128), as
-    ``kv_quantize_rows`` and decoding write them, with their slots' scales in ``k_scale``, ``v_scale`` [rows, Hkv, >= Smax]."""
+    ``kv_quantize_rows`` and decoding write them, with their slots' scales in ``k_scale``, ``v_scale`` [rows, Hkv, >= Smax].
+    Over these, nodes count with the keys and values of ``qkv`` as a prompt's tokens do, before they are rounded; with ``as_stored`` they count as
+    :func:`tree_accept` will store them, which is what decoding token by token sees."""
     if on_gpu(qkv):
-        o = native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale)
+        o = native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale, as_stored)
         tree.heads = Hq
         return o
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
@@ -98,6 +100,8 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
     if qkv.dtype != (torch.bfloat16 if fp8 else k_cache.dtype) and not (fp8 and qkv.dtype == torch.float32):
         raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}")
+    if as_stored and not fp8:
+        raise ValueError("only an fp8 cache stores nodes otherwise than they are")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
     if window < 0 or not 0 < scale < math.inf:
         raise ValueError(f"window {window}, scale {scale}")
@@ -109,7 +113,11 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     kv_start = None if kv_start is None else _ints(kv_start, "kv_start", (B,), qkv)
     if fp8:
         k_cache, v_cache = (kv_dequantize(c, sc[..., :Smax], k) for c, sc, k in ((k_cache, k_scale, True), (v_cache, v_scale, False)))
-    o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale)
+    kind = qkv.dtype
+    if as_stored:
+        q, *kv = qkv[:, :(Hq + 2 * Hkv) * D].float().split([Hq * D, Hkv * D, Hkv * D], 1)
+        qkv = torch.cat([q] + [kv_dequantize(*kv_quantize_rows(x.reshape(B * N, Hkv, D), k), k).view(B * N, Hkv * D) for x, k in zip(kv, (True, False))], 1)
+    o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale).to(kind)
     tree.heads = Hq
     return o if out is None else out.copy_(o)
 

@@ -140,3 +140,35 @@ def test_attention_refuses_an_output_of_another_shape(out):
         ops.tree_attention(torch.randn(2, 12), *(torch.randn(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 1, out=out)
     with pytest.raises(ValueError):
         ops.tree_attention(torch.randn(1, 12), *(torch.randn(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1]])), 1, out=out)
+
+
+# ------------------------------------------------------------------------------------------ nodes as an fp8 cache stores them
+def _two_heads(**kw):
+    cfg = models.ModelConfig(arch="mistral", vocab_size=64, hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, head_dim=128, intermediate_size=256,
+                             max_position=256, norm_eps=1e-5, name="two-heads")
+    return models.CausalLM(cfg, seed=1, **kw)
+
+
+def test_verify_as_stored_gives_the_states_of_decoding():
+    """a chain of drafts over an fp8 cache, and decoding it token by token over another one"""
+    m = _two_heads(dtype=torch.float32)
+    B, S, N = 2, 20, 12
+    g = torch.Generator().manual_seed(0)
+    ids, tokens = torch.randint(3, 60, (B, S), generator=g), torch.randint(3, 60, (B, N), generator=g)
+    start, kv_len = _i32([0, 15]), _i32([S, S])
+    a, b = (KVCache(2, B, 1, 64, 128, "cpu", torch.float32, fp8=True) for _ in "ab")
+    m.prefill(ids, start, a), m.prefill(ids, start, b)
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))] * B), pos0=kv_len - start)
+    h, drafts = m.verify(tokens, tree, kv_len, start, a, as_stored=True)
+    single = torch.stack([m.decode(tokens[:, i], kv_len - start + i, kv_len + i, kv_len + i + 1, start, b) for i in range(N)], 1)
+    assert torch.allclose(h.view(B, N, -1), single, rtol=1e-4, atol=1e-4)  # fp32 sums in other orders
+    plain, _ = m.verify(tokens, tree, kv_len, start, a)
+    assert not torch.allclose(plain.view(B, N, -1), single, rtol=1e-3, atol=1e-3)
+    ops.tree_accept(tree, tokens, torch.cat([tokens[:, 1:], tokens[:, :1]], 1), drafts, a.k, a.v, kv_len, a.ks, a.vs)
+    # a rounding may fall on the other side of a border where the states differ by fp32's roundings
+    assert (a.k != b.k).float().mean() < 1e-3 and (a.v != b.v).float().mean() < 1e-3
+
+
+def test_as_stored_wants_an_fp8_cache():
+    with pytest.raises(ValueError):
+        ops.tree_attention(torch.zeros(2, 12), *(torch.zeros(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 1, as_stored=True)

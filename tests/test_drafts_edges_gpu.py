@@ -263,3 +263,133 @@ def test_attention_beside_a_cache_in_one_allocation():
     cache = around[0, 304:304 + 1152].view(1, 2, 9, 64)  # at 16 bytes, as the other one: the same form
     cache.copy_(kc)
     assert torch.equal(_attend_into(around[:, :256], store[12000:12000 + 1024].view(2, 512).copy_(wide[:, :512]), cache, vc), want)
+
+
+# ------------------------------------------------------------------------------------------ nodes as an e4m3 cache stores them
+def _rounded(qkv, Hq, Hkv, D=128):
+    """rows with their keys and values as they are read back from an e4m3 cache, in fp32 on the CPU"""
+    x = qkv.float().cpu()
+    for at, key in ((Hq * D, True), ((Hq + Hkv) * D, False)):
+        x[:, at:at + Hkv * D] = ops.kv_dequantize(*ops.kv_quantize_rows(x[:, at:at + Hkv * D].reshape(-1, Hkv, D), key), key).reshape(-1, Hkv * D)
+    return x
+
+
+def _e4m3_cache(B, Hkv, slots, seed=0, D=128):
+    """-> (keys, values, their scales as arguments), and what they hold"""
+    held = [ops.kv_quantize_rows(torch.randn(B, Hkv, slots, D, generator=torch.Generator().manual_seed(seed + k)), k == 1) for k in (1, 2)]
+    (kq, ks), (vq, vs) = held
+    return [kq.to(DEV), vq.to(DEV)], dict(k_scale=ks.to(DEV), v_scale=vs.to(DEV)), [ops.kv_dequantize(kq, ks, True), ops.kv_dequantize(vq, vs, False)]
+
+
+def _tolerance(want, size, keys, D=128):
+    """the output's rounding, half a step; p times its scale rounded to bf16, half a step of each term; scores below 16 of D products and sums of 2^-24
+    each, the products with the scales, and as much again for the sums over the keys, exp2 and the division"""
+    half, fp32 = 2 ** -8, 2 * 2 ** -24 * (16 * (D + 2) + keys + 64)
+    return half * want.abs() + (half + fp32) * size * (1 + half)
+
+
+@pytest.mark.parametrize("Hq,Hkv,N", [(4, 4, 1), (5, 5, 16), (8, 2, 8), (32, 8, 16), (8, 2, 33), (8, 2, 64), (12, 1, 64)])
+@pytest.mark.parametrize("window", [0, 3, 50])
+def test_attention_as_stored(Hq, Hkv, N, window):
+    lens, starts, counts = [130, 0, 1, 64, 65, 191], [0, 0, 0, 10, 64, 3], [N, N, N, 1, N, 0]
+    B, D, slots = len(lens), 128, 200
+    parents = plain.trees(B, N, N)
+    qkv = _rand(B * N, (Hq + 2 * Hkv) * D, seed=N)
+    (kq, vq), scales, (kc, vc) = _e4m3_cache(B, Hkv, slots, N)
+    for b in range(B):  # no numbers where nothing is seen
+        qkv[b * N + counts[b]:(b + 1) * N] = math.nan
+        for c, sc in ((kq, scales["k_scale"]), (vq, scales["v_scale"])):
+            for part in (slice(0, starts[b]), slice(lens[b], slots)):
+                c[b, :, part], sc[b, :, part] = 0x7f, math.nan
+    out = torch.full((B * N, Hq * D), 7.0, dtype=BF16, device=DEV)
+    ops.tree_attention(qkv, kq, vq, _i32(lens), ops.draft_tree(_i32(parents), _i32(counts)), Hq, _i32(starts), window, out=out, as_stored=True, **scales)
+    want, size = plain.attention(_rounded(torch.nan_to_num(qkv), Hq, Hkv), kc, vc, lens, parents, counts, Hq, starts, window)
+    err, tol = (out.cpu().double() - want).abs(), _tolerance(want, size, 200 + N)
+    assert (err <= tol).all(), f"worst {(err / tol.clamp(min=1e-30)).max().item():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("lens", [[2100], [900, 9, 700]])
+@pytest.mark.parametrize("N", [2, 30, 60])
+def test_attention_as_stored_over_a_long_cache(lens, N):
+    B, Hq, Hkv, D = len(lens), 8, 2, 128
+    parents = plain.trees(B, N, N)
+    wide = _rand(B * N, (Hq + 2 * Hkv) * D + 3, seed=N)  # rows of an odd pitch
+    (kq, vq), scales, (kc, vc) = _e4m3_cache(B, Hkv, max(lens) + 5, N)
+    got = ops.tree_attention(wide, kq, vq, _i32(lens), ops.draft_tree(_i32(parents)), Hq, as_stored=True, **scales)
+    want, size = plain.attention(_rounded(wide, Hq, Hkv), kc, vc, lens, parents, [N] * B, Hq)
+    assert ((got.cpu().double() - want).abs() <= _tolerance(want, size, max(lens) + N)).all()
+
+
+def test_attention_as_stored_does_not_depend_on_how_much_is_drafted():
+    """a chain at once, and its second half after the first one was appended"""
+    Hq, Hkv, D, N, half, n = 8, 2, 128, 40, 17, 70
+    qkv = _rand(N, (Hq + 2 * Hkv) * D)
+    (kq, vq), scales, (kc, vc) = _e4m3_cache(1, Hkv, 200)
+    chain = [-1] + list(range(N - 1))
+    at_once = ops.tree_attention(qkv, kq, vq, _i32([n]), ops.draft_tree(_i32([chain])), Hq, as_stored=True, **scales)[half:]
+    first = ops.draft_tree(_i32([chain[:half]]))
+    tokens = torch.arange(half, device=DEV)[None]
+    count, _, _ = ops.tree_accept(first, tokens, tokens + 1, [qkv[:half]], kq[None], vq[None], _i32([n]), scales["k_scale"][None], scales["v_scale"][None])
+    assert int(count) == half
+    later = ops.tree_attention(qkv[half:], kq, vq, _i32([n + half]), ops.draft_tree(_i32([chain[:N - half]])), Hq, as_stored=True, **scales)
+    want, size = (t[half:] for t in plain.attention(_rounded(qkv, Hq, Hkv), kc, vc, [n], [chain], [N], Hq))
+    for got in (at_once, later):
+        assert ((got.cpu().double() - want).abs() <= _tolerance(want, size, n + N)).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("Hq,Hkv", [(2, 2), (8, 2), (8, 1), (32, 1)])
+def test_attention_as_stored_keeps_nodes_apart(Hq, Hkv, bad):
+    """values that are no numbers in one branch, all of a row or one element of it, leave the other branches as they are"""
+    N, D = 20, 128
+    parents = [[-1, 0, 0] + list(range(1, N - 2))]  # two chains from the root: odd and even nodes
+    qkv = _rand(N, (Hq + 2 * Hkv) * D)
+    qkv[7].view(-1, D)[Hq + Hkv:, 5] = 0
+    (kq, vq), scales, _ = _e4m3_cache(1, Hkv, 70)
+    run = lambda: ops.tree_attention(qkv, kq, vq, _i32([66]), ops.draft_tree(_i32(parents)), Hq, as_stored=True, **scales)
+    want = run()
+    ill = [i for i, f in enumerate(plain.chains(parents[0], N)) if 7 in f]
+    well = [i for i in range(N) if i not in ill]
+    qkv[7].view(-1, D)[Hq + Hkv:, 5] = bad
+    got = run()
+    assert torch.equal(got[well], want[well])
+    of, ref = got[ill].view(len(ill), Hq, D), want[ill].view(len(ill), Hq, D)
+    if math.isnan(bad):  # that element alone; an infinite one has the whole row in its scale
+        assert torch.isnan(of[:, :, 5]).all()
+        of[:, :, 5] = ref[:, :, 5]
+        assert torch.equal(of, ref)
+    else:
+        assert torch.isnan(of).all()
+    qkv[7, Hq * D:] = bad
+    got = run()
+    assert torch.equal(got[well], want[well]) and torch.isnan(got[ill]).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_model_checks_drafts_as_stored_like_single_steps(fp8):
+    """hidden states of a chain of drafts and those of decoding it token by token"""
+    cfg = models.ModelConfig(arch="mistral", vocab_size=64, hidden_size=256, num_layers=2, num_heads=2, num_kv_heads=1, head_dim=128, intermediate_size=256,
+                             max_position=256, norm_eps=1e-5, name="two-heads")
+    m = models.CausalLM(cfg, device=DEV, dtype=BF16, seed=1)
+    B, S, N = 2, 20, 32
+    ids = torch.randint(3, 60, (B, S), generator=torch.Generator().manual_seed(0)).to(DEV)
+    start, kv_len = _i32([0, 15]), _i32([S, S])
+    a, b = (KVCache(2, B, 1, 128, 128, DEV, fp8=fp8) for _ in "ab")
+    m.prefill(ids, start, a), m.prefill(ids, start, b)
+    tokens = torch.randint(3, 60, (B, N), generator=torch.Generator().manual_seed(1)).to(DEV)
+    tree = ops.draft_tree(_i32([[-1] + list(range(N - 1))] * B), pos0=kv_len - start)
+    h, drafts = m.verify(tokens, tree, kv_len, start, a, as_stored=True)
+    single = torch.stack([m.decode(tokens[:, i], kv_len - start + i, kv_len + i, kv_len + i + 1, start, b) for i in range(N)], 1)
+    x, y = h.view(B, N, -1).float(), single.float()
+    # normalised states, each of about 16 roundings to bf16 on its way through two layers. In e4m3 such a difference d of a key or value crosses
+    # a border of its steps (2^-3) with probability d / 2^-3 and moves it by the step: a variance of 2^-3 d, of d = 4 x 2^-8 here, over at least five keys
+    var = 16 * 2 ** -16 + (2 ** -3 * 4 * 2 ** -8 / 5 if fp8 else 0)
+    assert (x - y).pow(2).mean().sqrt() <= var ** 0.5 * y.pow(2).mean().sqrt()
+    if fp8:  # the states of attending to unrounded drafts are further away
+        z = m.verify(tokens, tree, kv_len, start, a)[0].view(B, N, -1).float()
+        assert (x - y).pow(2).mean() < (z - y).pow(2).mean()
+
+
+def test_as_stored_wants_an_e4m3_cache():
+    with pytest.raises(ValueError):
+        ops.tree_attention(_rand(2, 512), *(_rand(1, 2, 9, 64) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, as_stored=True)
