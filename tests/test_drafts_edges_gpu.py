@@ -393,3 +393,62 @@ def test_a_model_checks_drafts_as_stored_like_single_steps(fp8):
 def test_as_stored_wants_an_e4m3_cache():
     with pytest.raises(ValueError):
         ops.tree_attention(_rand(2, 512), *(_rand(1, 2, 9, 64) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 4, as_stored=True)
+
+
+# ------------------------------------------------------------------------------------------ rows taken in another order
+def _mixed(B, slots, seed):
+    """lengths in no order, with equal ones, none, one, all, and some that do not fit"""
+    r = torch.randint(0, slots, (B,), generator=torch.Generator().manual_seed(seed)).tolist()
+    special = [0, 0, 1, slots, slots, slots + 7, 2 ** 31 - 1, -1, -2 ** 31, 64, 64, 64, 63, 65, slots - 1]
+    return [special[i // 2] if i % 2 and i // 2 < len(special) else n for i, n in enumerate(r)]
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,N,fp8", [(64, 32, 8, 128, 50, False), (63, 32, 8, 128, 64, False), (63, 64, 8, 128, 40, False), (64, 32, 8, 64, 64, False),
+                                              (40, 64, 8, 64, 33, False), (64, 32, 8, 128, 50, True), (63, 32, 8, 128, 64, True), (63, 64, 8, 128, 40, True)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_a_row_is_the_same_in_a_batch_that_is_taken_by_length(B, Hq, Hkv, D, N, fp8, window):
+    """more rows of 192 queries a key head than the card takes at once go by their lengths: each gives the bits that it gives beside one other row"""
+    slots = 150
+    lens, counts = _mixed(B, slots, B), [0 if i % 9 == 4 else N - i % (N // 2) for i in range(B)]
+    starts = [(7 * i) % 31 for i in range(B)]
+    parents = plain.trees(B, N, B)
+    qkv = _rand(B * N, (Hq + 2 * Hkv) * D, seed=1)
+    if fp8:
+        held, scales, _ = _e4m3_cache(B, Hkv, slots)
+    else:
+        held, scales = [_rand(B, Hkv, slots, D, seed=k) for k in (2, 3)], {}
+
+    def run(rows):
+        out = torch.full((len(rows) * N, Hq * D), 7.0, dtype=BF16, device=DEV)
+        pick = lambda x: [x[i] for i in rows]
+        at = torch.tensor(rows, device=DEV)
+        ops.tree_attention(qkv.view(B, N, -1)[at].view(len(rows) * N, -1), *(c[at] for c in held), _i32(pick(lens)), ops.draft_tree(_i32(pick(parents)), _i32(pick(counts))),
+                           Hq, _i32(pick(starts)), window, out=out, **{k: v[at] for k, v in scales.items()})
+        return out.view(len(rows), N, -1)
+
+    whole = run(list(range(B)))
+    for i in range(0, B - 1, 2):
+        assert torch.equal(whole[i:i + 2], run([i, i + 1])), (i, lens[i:i + 2], counts[i:i + 2])
+    assert torch.equal(whole[-2:], run([B - 2, B - 1]))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_long_rows_in_parts_taken_by_length(fp8):
+    """rows that are cut into parts and taken by their lengths"""
+    B, Hq, Hkv, D, N, slots = 25, 16, 4, 128, 50, 3000
+    lens = [(i * 37) % 41 for i in range(B)]
+    lens[3], lens[9], lens[10], lens[17], lens[24] = 2900, 3000, 1200, 2900, 700
+    counts = [N if i in (3, 24) else i % 4 for i in range(B)]
+    counts[9], counts[10], counts[17] = 3, 1, 0
+    parents = plain.trees(B, N, 1)
+    qkv = _rand(B * N, (Hq + 2 * Hkv) * D, seed=1)
+    if fp8:
+        held, scales, (kc, vc) = _e4m3_cache(B, Hkv, slots)
+    else:
+        held, scales = [_rand(B, Hkv, slots, D, seed=k) for k in (2, 3)], {}
+        kc, vc = held
+    out = torch.full((B * N, Hq * D), 7.0, dtype=BF16, device=DEV)
+    ops.tree_attention(qkv, *held, _i32(lens), ops.draft_tree(_i32(parents), _i32(counts)), Hq, out=out, **scales)
+    want, size = plain.attention(qkv, kc, vc, lens, parents, counts, Hq)
+    err, tol = (out.cpu().double() - want).abs(), _tolerance(want, size, slots + N)
+    assert (err <= tol).all(), f"worst {(err / tol.clamp(min=1e-30)).max().item():.2f} of the tolerance"
