@@ -484,7 +484,8 @@ class CausalLM(nn.Module):
         cfg = self.cfg
         kv8 = getattr(cache, "fp8", False)
         cos, sin = self.rope(tokens.device)
-        tree.see.masked_fill_(tree.pos >= cfg.max_position, 0)
+        with torch.inference_mode():  # wherever the plan was made
+            tree.see.masked_fill_(tree.pos >= cfg.max_position, 0)
         # what is no node may hold any token (an idle row's next one is -1) and any position
         pos = tree.pos.reshape(-1).clamp(0, cfg.max_position - 1)
         x = self.embed_tokens(torch.where(tree.see != 0, tokens, 0).reshape(-1), pos)

@@ -172,3 +172,12 @@ def test_verify_as_stored_gives_the_states_of_decoding():
 def test_as_stored_wants_an_fp8_cache():
     with pytest.raises(ValueError):
         ops.tree_attention(torch.zeros(2, 12), *(torch.zeros(1, 1, 9, 4) for _ in "kv"), _i32([3]), ops.draft_tree(_i32([[-1, 0]])), 1, as_stored=True)
+
+
+def test_verify_of_a_plan_made_in_inference_mode():
+    m = models.CausalLM(models.resolve_preset("tiny-opt"), dtype=torch.float32, seed=3)
+    cache = KVCache(m.cfg.num_layers, 1, m.cfg.num_kv_heads, 16, m.cfg.head_dim, "cpu", torch.float32)
+    with torch.inference_mode():
+        tree = ops.draft_tree(_i32([[-1, 0]]), pos0=_i32([3]))
+    h, _ = m.verify(torch.tensor([[5, 6]]), tree, _i32([3]), None, cache)
+    assert torch.isfinite(h).all()
