@@ -73,7 +73,7 @@ bool apart(const Span& a, const Span& b) {
   return col >= b.width && col + a.width <= a.pitch;
 }
 // layers that are written at once: each has memory of its own
-bool layers_apart(const Tensor& t) { return t.size(0) <= 1 || !t.numel() || t.stride(0) >= t[0].numel(); }
+bool layers_apart(const Tensor& t) { return t.size(0) <= 1 || !t.numel() || t.stride(0) >= t.numel() / t.size(0); }
 
 // the slots' scales of an e4m3 cache [.., rows, heads, slots, 128], alike for keys and values
 struct Scales { float* k = nullptr; float* v = nullptr; long layer = 0; int slots = 0; };
@@ -185,18 +185,22 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
               "tree_accept: caches of one type and layout, contiguous in each layer");
   const Scales sc = scales(kc, k_scale, v_scale);
   TORCH_CHECK_VALUE(layers_apart(kc) && (!sc.k || layers_apart(*k_scale)), "tree_accept: layers of one memory");
-  TORCH_CHECK_VALUE(apart(span(kc), span(vc)) && (!sc.k || apart(span(*k_scale), span(*v_scale))), "tree_accept: keys and values of one memory");
+  const Span keys = span(kc), values = span(vc);
+  TORCH_CHECK_VALUE(apart(keys, values) && (!sc.k || apart(span(*k_scale), span(*v_scale))), "tree_accept: keys and values of one memory");
   const Tensor kv_len = ints(kv_len_, at::kInt, {B}, kc, "kv_len");
   whole(parent, at::kInt, {B, N}, kc, "tree_accept tree");
   whole(see, at::kLong, {B, N}, kc, "tree_accept tree");
   const Tensor tokens = ints(tokens_, at::kLong, {B, N}, kc, "tokens"), choice = ints(choice_, at::kLong, {B, N}, kc, "choice");
   bool copy = false;  // e4m3: rows at 16 bytes, others are copied
+  const int64_t bytes = drafts[0].dim() == 2 && drafts[0].numel()
+                            ? ((drafts[0].size(0) - 1) * drafts[0].stride(0) + drafts[0].size(1)) * drafts[0].element_size() : 0;  // alike, see below
   for (const Tensor& x : drafts) {
     on(x, kc, "tree_accept drafts");
     TORCH_CHECK_VALUE(x.scalar_type() == (sc.k ? at::kBFloat16 : kc.scalar_type()) && x.dim() == 2 && x.stride(1) == 1 && x.sizes() == drafts[0].sizes() &&
                     x.stride(0) == drafts[0].stride(0) && x.size(0) == B * N,
                 "tree_accept: drafts [rows nodes, (heads + 2 key heads) dim] of the caches' type, alike in every layer");
-    TORCH_CHECK_VALUE(apart(span(x), span(kc)) && apart(span(x), span(vc)), "tree_accept: drafts in the caches' memory");
+    const char* const from = (const char*)x.data_ptr();
+    TORCH_CHECK_VALUE(!bytes || (apart(from, from + bytes, keys) && apart(from, from + bytes, values)), "tree_accept: drafts in the caches' memory");
     copy = copy || (sc.k && (!al(x, 16) || x.stride(0) % 8));
   }
   // keys lie behind `heads` queries; where nobody said how many (0), the rows hold nothing behind [q | k | v]

@@ -5,7 +5,6 @@
 #include "rt_paged.h"
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -289,7 +288,8 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
   if (rb * ROWS < M) {
     bf16x8 qf[RT][DS];
     uint64_t sees[RT];
-    int from[RT];  // first key of the context that the row sees; of rows that are no nodes one behind all
+    int from[RT];       // first key of the context that the row sees
+    bool sees_any[RT];  // set in steps, as a mask of the wave: as one expression it costs the loop below registers (64 rows of 64 nodes 194 -> 197 us)
     const int joint = !KV8 && ct.tiles == ct.full + 1 ? ct.rest : 0;
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
@@ -298,10 +298,12 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
 #pragma unroll
       for (int d = 0; d < DS; ++d) qf[u][d] = *(const bf16x8*)(q + 32 * d);
       const uint64_t w = lane64(see, node);
-      from[u] = !w ? INT_MAX : a.window ? ct.len + (int)__popcll(w) - a.window : 0;
+      sees_any[u] = w != 0;
+      from[u] = a.window ? ct.len + (int)__popcll(w) - a.window : 0;
       // by the nodes' stage: its first `joint` keys are the context's last ones
       const uint64_t ctx = ~0ull << min(max(from[u] - (ct.len - joint), 0), 63) & ((1ull << joint) - 1);  // joint is 63 at most
       sees[u] = near_nodes(w, see, a.window) << joint | ctx;
+      if (a.window && !sees[u] && max(from[u], ct.lo) >= ct.len) sees_any[u] = false;
     }
     f32x4 o[RT][DT];
     float m[RT], l[RT];
@@ -764,12 +766,11 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
         for (int c = 0; c < DT; ++c) q[64 * c] = o[u][c];
       } else if (r < M) {
         const float inv = 1.f / l[u];
-        const bool sees_any = sees[u] || max(from[u], ct.lo) < ct.len;
         const int node = node_of_row(a, r);
         bf16_t* const p = (bf16_t*)a.o + ((long)b * a.N + node) * a.ldo + (long)(gh * G + r - node * G) * D + 4 * g;
 #pragma unroll
         for (int c = 0; c < DT; ++c)
-          *(uint2*)(p + 16 * c) = sees_any ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
+          *(uint2*)(p + 16 * c) = sees_any[u] ? make_uint2(pack2bf(o[u][c][0] * inv, o[u][c][1] * inv), pack2bf(o[u][c][2] * inv, o[u][c][3] * inv))
                                           : make_uint2(0, 0);
       }
     }
