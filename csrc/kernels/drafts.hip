@@ -251,7 +251,7 @@ __device__ __forceinline__ float largest16(float x) {
 // a value of a row with this scale, as the row is read once it lies in an e4m3 cache
 __device__ __forceinline__ float as_stored(float v, float scale) { return fp8_at(__builtin_amdgcn_cvt_pk_fp8_f32(v * (1.f / scale), 0.f, 0, false), 0) * scale; }
 
-// The bound: 128 registers where two workgroups of eight waves share a CU (in e4m3, with 162: rows of 128 queries 91 us, with the bound 81); elsewhere 256,
+// The bound: 128 registers where two workgroups of eight waves share a CU (in e4m3, with 162: rows of 128 queries took an eighth more); elsewhere 256,
 // without which the compiler keeps some in the matrix cores' file and moves them in each stage (32 rows of 5 nodes, 12 heads of 64: 11.3 us, with
 // it 10.7; 64 rows of 64 nodes 209 and 205).
 // STORED: the nodes' keys and values count as they will be once they lie in the e4m3 cache.
@@ -363,10 +363,10 @@ __global__ __launch_bounds__(64 * WR * WK, WR == 4 ? 4 : 2) void tree_mfma_kerne
       }
     };
     // An e4m3 cache: its stages go to LDS as they are, in a ring of four, three under way, and become bf16 (exact) where fragments are read.
-    // The nodes' stage, in bf16, takes the half of the ring that the last of these is not in. Measured against a cache in bf16: 64 rows of 48 nodes
-    // over 100 to 700 keys in 32 key heads of one query each 74 us for 93, 16 rows of 32 nodes 37 for 46, where memory bounds these; 48 rows of 16 nodes in
-    // 8 heads of four 35 for 29, and 64 rows of 64 nodes over 1000 to 4000 keys 233 for 204, where the instructions do: each wave converts what it
-    // reads. (Converted once, in a pass over LDS with a barrier: 77, 49, 38, 230.)
+    // The nodes' stage, in bf16, takes the half of the ring that the last of these is not in. Measured against a cache in bf16, captured: 64 rows of
+    // 48 nodes over 100 to 700 keys in 32 key heads of one query each 74 us for 92, 16 rows of 32 nodes 37 for 45, where memory bounds these; 48 rows of 16
+    // nodes in 8 heads of four 36 for 30, and 64 rows of 64 nodes over 1000 to 4000 keys 222 for 206 to 219 (by the card's power), where the instructions
+    // do: each wave converts what it reads. (Converted once, in a pass over LDS with a barrier, the first three took 77, 49 and 38.)
     const int raw_end = min(t1, ct.tiles - 1);
     auto fetch = [&](int tile) {
       const int last = ct.len - ct.lo - tile * SK - 1, slot = tile - t0 & 3;
