@@ -108,6 +108,10 @@ optional<Tensor> ints(const optional<Tensor>& t, at::ScalarType type, at::IntArr
   return ints(*t, type, shape, like, n);
 }
 
+// What a tree was read with, by key heads, head size and columns of the rows: query heads, or None where not always as many. The
+// plain form in Python makes the same keys.
+py::int_ rows_of(int64_t Hkv, int64_t D, int64_t cols) { return py::int_(Hkv >> 16 || D >> 17 || cols >> 30 ? -1 : (Hkv << 17 | D) << 30 | cols); }
+
 std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parent_, const optional<Tensor>& nodes_, const optional<Tensor>& pos0_) {
   TORCH_CHECK_VALUE(parent_.is_cuda() && parent_.dim() == 2 && parent_.size(1) >= 1 && parent_.size(1) <= 64,
                     "parent: [rows, 1 .. 64 nodes] expected, got ", parent_.sizes());
@@ -123,7 +127,7 @@ std::tuple<Tensor, Tensor, Tensor> draft_tree(const Tensor& parent_, const optio
 
 Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, const Tensor& kv_len_, const optional<Tensor>& kv_start_,
                       const Tensor& see, const optional<Tensor>& out_, int64_t Hq, int64_t window, const optional<double>& scale_,
-                      const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, bool as_stored) {
+                      const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, bool as_stored, const py::dict& heads) {
   act(qkv, "tree_attention qkv");
   TORCH_CHECK_VALUE(kc.dim() == 4 && see.dim() == 2 && qkv.dim() == 2 && (qkv.stride(1) == 1 || qkv.size(0) == 0),
                     "tree_attention: qkv [rows nodes, columns], caches [rows, heads, slots, dim] expected, got ", qkv.sizes(), ", ", kc.sizes());
@@ -142,7 +146,7 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
                     " heads over ", Hkv, " of ", D, " and ", B, " rows of ", N, " nodes do not fit qkv ", qkv.sizes());
   const double scale = scale_.has_value() ? *scale_ : 1 / std::sqrt((double)D);
   TORCH_CHECK_VALUE(window >= 0 && scale > 0 && std::isfinite(scale), "tree_attention: window ", window, ", scale ", scale);
-  TORCH_CHECK_VALUE(D <= 512 && Smax * D < (1L << 30) && window < (1L << 30) && Hq < 65536 && B < 65536, "tree_attention: sizes");
+  TORCH_CHECK_VALUE(D <= 512 && qkv.size(1) < (1L << 30) && Smax * D < (1L << 30) && window < (1L << 30) && Hq < 65536 && B < 65536, "tree_attention: sizes");
   TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(qkv.requires_grad() || kc.requires_grad() || vc.requires_grad()),
                     "tree_attention has no gradient");
   const c10::DeviceGuard guard(qkv.device());
@@ -167,12 +171,16 @@ Tensor tree_attention(const Tensor& qkv, const Tensor& kc, const Tensor& vc, con
                           kv_len.data_ptr<int>(), ptr<int>(kv_start), see.data_ptr<int64_t>(), o.data_ptr(), o.stride(0), S > 1 ? part.data_ptr<float>() : nullptr,
                           (int)S, (int)B, (int)N, (int)Hq, (int)Hkv, (int)D, (int)Smax, (int)window, (float)scale, as_stored, stream()), "tree_attention");
   if (!o.is_same(out)) out.copy_(o);
+  const py::int_ rows = rows_of(Hkv, D, qkv.size(1)), read(Hq);
+  PyObject* const before = PyDict_SetDefault(heads.ptr(), rows.ptr(), read.ptr());
+  if (!before) throw py::error_already_set();
+  if (before != Py_None && PyLong_AsLongLong(before) != Hq) heads[rows] = py::none();
   return out;
 }
 
 std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tensor& see, const Tensor& tokens_, const Tensor& choice_,
                                                const std::vector<Tensor>& drafts, Tensor kc, Tensor vc, const Tensor& kv_len_,
-                                               const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, int64_t heads) {
+                                               const optional<Tensor>& k_scale, const optional<Tensor>& v_scale, int64_t heads, const py::dict& read) {
   if (!has(k_scale)) act(kc, "tree_accept k_cache");
   TORCH_CHECK_VALUE(kc.is_cuda(), "tree_accept k_cache: GPU tensor expected");
   TORCH_CHECK_VALUE(kc.dim() == 5 && see.dim() == 2 && drafts.size() && (int64_t)drafts.size() == kc.size(0) && drafts.size() <= 256,
@@ -203,8 +211,14 @@ std::tuple<Tensor, Tensor, Tensor> tree_accept(const Tensor& parent, const Tenso
     TORCH_CHECK_VALUE(!bytes || (apart(from, from + bytes, keys) && apart(from, from + bytes, values)), "tree_accept: drafts in the caches' memory");
     copy = copy || (sc.k && (!al(x, 16) || x.stride(0) % 8));
   }
-  // keys lie behind `heads` queries; where nobody said how many (0), the rows hold nothing behind [q | k | v]
-  const int64_t cols = drafts[0].size(1), Hq = heads ? heads : cols / D - 2 * Hkv;
+  // keys lie behind `heads` queries; where nobody said how many (0), as tree_attention read such rows, or the rows hold nothing behind [q | k | v]
+  const int64_t cols = drafts[0].size(1);
+  if (!heads) {
+    PyObject* const before = PyDict_GetItem(read.ptr(), rows_of(Hkv, D, cols).ptr());
+    TORCH_CHECK_VALUE(before != Py_None, "tree_accept: rows of this width were read with different heads: Hq says which these have");
+    if (before) heads = PyLong_AsLongLong(before);
+  }
+  const int64_t Hq = heads ? heads : cols / D - 2 * Hkv;
   TORCH_CHECK_VALUE(Hq > 0 && Hq % Hkv == 0 && Hq < 65536 && cols >= (Hq + 2 * Hkv) * D && (heads || cols % D == 0), "tree_accept: ", Hq,
                     " heads over ", Hkv, " of ", D, " do not fit drafts of ", cols, " columns");
   std::vector<const void*> at;

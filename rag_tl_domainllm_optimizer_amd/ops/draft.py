@@ -8,7 +8,7 @@ accepted never touch the cache. All of it stays on the device and can be capture
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import List, Optional
 
 import torch
@@ -23,12 +23,13 @@ MAX_NODES = 64  # a node's ancestors are the bits of one word
 @dataclass
 class DraftTree:
     """Trees of a batch, [rows, nodes] each: parent int32 (as given), see int64 (bit j: the node itself or its ancestor j; 0: not
-    a node), pos int32. ``heads``: query heads of the rows that :func:`tree_attention` read with it (0: none yet)."""
+    a node), pos int32. ``heads``: of rows that :func:`tree_attention` read with it, by key heads, head size and columns, the query heads (None: not
+    always as many)."""
 
     parent: torch.Tensor
     see: torch.Tensor
     pos: torch.Tensor
-    heads: int = 0
+    heads: dict = field(default_factory=dict)
 
     @property
     def shape(self):
@@ -55,6 +56,10 @@ def _scales(k_cache, v_cache, k_scale, v_scale) -> bool:
 def _nodes(tree):
     if tree.see.dim() != 2 or not 1 <= tree.see.shape[1] <= MAX_NODES:
         raise ValueError(f"a tree [rows, 1 .. {MAX_NODES} nodes] expected, got {tuple(tree.shape)}")
+
+
+def _rows_of(Hkv, D, cols):
+    return -1 if Hkv >> 16 or D >> 17 or cols >> 30 else (Hkv << 17 | D) << 30 | cols
 
 
 def draft_tree(parent: torch.Tensor, nodes: Optional[torch.Tensor] = None, pos0: Optional[torch.Tensor] = None) -> DraftTree:
@@ -85,9 +90,7 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Over these, nodes count with the keys and values of ``qkv`` as a prompt's tokens do, before they are rounded; with ``as_stored`` they count as
     :func:`tree_accept` will store them, which is what decoding token by token sees."""
     if on_gpu(qkv):
-        o = native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale, as_stored)
-        tree.heads = Hq
-        return o
+        return native().tree_attention(qkv, k_cache, v_cache, kv_len, kv_start, tree.see, out, Hq, window, scale, k_scale, v_scale, as_stored, tree.heads)
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise ValueError(f"caches [rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     _nodes(tree)
@@ -118,7 +121,11 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         q, *kv = qkv[:, :(Hq + 2 * Hkv) * D].float().split([Hq * D, Hkv * D, Hkv * D], 1)
         qkv = torch.cat([q] + [kv_dequantize(*kv_quantize_rows(x.reshape(B * N, Hkv, D), k), k).view(B * N, Hkv * D) for x, k in zip(kv, (True, False))], 1)
     o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale).to(kind)
-    tree.heads = Hq
+    key = _rows_of(Hkv, D, qkv.shape[1])
+    if key < 0:
+        raise ValueError(f"{Hkv} key heads of {D} in {qkv.shape[1]} columns")
+    if tree.heads.setdefault(key, Hq) != Hq:
+        tree.heads[key] = None
     return o if out is None else out.copy_(o)
 
 
@@ -131,13 +138,12 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
     (per layer the rows that :func:`tree_attention` read) to the slots from ``kv_len`` of the caches [layers, rows, Hkv, Smax, D]; ``kv_len``
     itself is the caller's to advance by the length. An idle row has length 0 and token -1. A path ends
     with the cache: its last node is the one that took the last slot, the token the choice after that; a row without a slot idles.
-    ``Hq``: query heads in front of the keys in ``drafts``, by default as :func:`tree_attention` read them with this tree; before it did, rows
+    ``Hq``: query heads in front of the keys in ``drafts``, by default as :func:`tree_attention` read rows of this width with this tree; others
     hold nothing behind [q | k | v]. ``k_scale`` / ``v_scale`` [layers, rows, Hkv, >= Smax]: the caches are fp8, and rows are rounded into them as ``kv_store_fp8`` does."""
     if Hq is not None and Hq < 1:
         raise ValueError(f"{Hq} query heads")
-    heads = tree.heads if Hq is None else Hq
     if on_gpu(k_cache):
-        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale, heads)
+        return native().tree_accept(tree.parent, tree.see, tokens, choice, drafts, k_cache, v_cache, kv_len, k_scale, v_scale, Hq or 0, tree.heads)
     if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
         raise ValueError(f"caches [layers, rows, heads, slots, dim] expected, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     _nodes(tree)
@@ -157,6 +163,9 @@ def tree_accept(tree: DraftTree, tokens: torch.Tensor, choice: torch.Tensor, dra
                                for x in drafts):
         raise ValueError(f"drafts: rows [q | k | v] of {B * tree.shape[1]} nodes in {k_cache.dtype} for each of {L} layers expected")
     cols = drafts[0].shape[1]
+    heads = tree.heads.get(_rows_of(Hkv, D, cols), 0) if Hq is None else Hq
+    if heads is None:
+        raise ValueError("rows of this width were read with different heads: Hq says which these have")
     Hq = heads or cols // D - 2 * Hkv
     if Hq < 1 or Hq % Hkv or cols < (Hq + 2 * Hkv) * D or (not heads and cols % D):
         raise ValueError(f"{Hq} heads over {Hkv} of {D} do not fit drafts of {cols} columns")

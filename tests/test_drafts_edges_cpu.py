@@ -181,3 +181,25 @@ def test_verify_of_a_plan_made_in_inference_mode():
         tree = ops.draft_tree(_i32([[-1, 0]]), pos0=_i32([3]))
     h, _ = m.verify(torch.tensor([[5, 6]]), tree, _i32([3]), None, cache)
     assert torch.isfinite(h).all()
+
+
+def test_accept_after_two_models_read_the_tree():
+    """the heads are those of rows of the drafts' width; where one width was read with different heads, the caller says which"""
+    N, D, slots = 3, 4, 9
+    tree, tokens = ops.draft_tree(_i32([[-1, 0, 1]])), torch.arange(N)[None]
+    g = torch.Generator().manual_seed(0)
+    a, b = (torch.randn(N, (Hq + 2) * D, generator=g) for Hq in (4, 2))
+    cache = lambda L: (torch.zeros(L, 1, 1, slots, D), torch.zeros(L, 1, 1, slots, D))
+    for rows, Hq in ((a, 4), (b, 2)):
+        kc, vc = cache(1)
+        ops.tree_attention(rows, kc[0], vc[0], _i32([0]), tree, Hq)
+    for rows, Hq in ((a, 4), (b, 2)):
+        kc, vc = cache(1)
+        ops.tree_accept(tree, tokens, tokens + 1, [rows], kc, vc, _i32([0]))
+        assert torch.equal(kc[0, 0, 0, :N], rows[:, Hq * D:(Hq + 1) * D]) and torch.equal(vc[0, 0, 0, :N], rows[:, (Hq + 1) * D:])
+    kc, vc = cache(1)
+    ops.tree_attention(a, kc[0], vc[0], _i32([0]), tree, 2)
+    with pytest.raises(ValueError):
+        ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]))
+    ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]), Hq=2)
+    assert torch.equal(kc[0, 0, 0, :N], a[:, 2 * D:3 * D])

@@ -452,3 +452,24 @@ def test_long_rows_in_parts_taken_by_length(fp8):
     want, size = plain.attention(qkv, kc, vc, lens, parents, counts, Hq)
     err, tol = (out.cpu().double() - want).abs(), _tolerance(want, size, slots + N)
     assert (err <= tol).all(), f"worst {(err / tol.clamp(min=1e-30)).max().item():.2f} of the tolerance"
+
+
+def test_accept_after_two_models_read_the_tree():
+    """the heads are those of rows of the drafts' width; where one width was read with different heads, the caller says which"""
+    N, D, slots = 3, 64, 9
+    tree, tokens = ops.draft_tree(_i32([[-1, 0, 1]])), torch.arange(N, device=DEV)[None]
+    a, b = (_rand(N, (Hq + 2) * D, seed=Hq) for Hq in (4, 2))
+    cache = lambda: [torch.zeros(1, 1, 1, slots, D, dtype=BF16, device=DEV) for _ in "kv"]
+    for rows, Hq in ((a, 4), (b, 2)):
+        kc, vc = cache()
+        ops.tree_attention(rows, kc[0], vc[0], _i32([0]), tree, Hq)
+    for rows, Hq in ((a, 4), (b, 2)):
+        kc, vc = cache()
+        ops.tree_accept(tree, tokens, tokens + 1, [rows], kc, vc, _i32([0]))
+        assert torch.equal(kc[0, 0, 0, :N], rows[:, Hq * D:(Hq + 1) * D]) and torch.equal(vc[0, 0, 0, :N], rows[:, (Hq + 1) * D:])
+    kc, vc = cache()
+    ops.tree_attention(a, kc[0], vc[0], _i32([0]), tree, 2)
+    with pytest.raises(ValueError):
+        ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]))
+    ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]), Hq=2)
+    assert torch.equal(kc[0, 0, 0, :N], a[:, 2 * D:3 * D])
