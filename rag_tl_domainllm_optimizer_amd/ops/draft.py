@@ -103,6 +103,9 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     fp8 = _scales(k_cache, v_cache, k_scale, v_scale)
     if qkv.dtype != (torch.bfloat16 if fp8 else k_cache.dtype) and not (fp8 and qkv.dtype == torch.float32):
         raise ValueError(f"caches of {k_cache.dtype} under queries of {qkv.dtype}")
+    key = _rows_of(Hkv, D, qkv.shape[1])
+    if key < 0:
+        raise ValueError(f"{Hkv} key heads of {D} in {qkv.shape[1]} columns")
     if as_stored and not fp8:
         raise ValueError("only an fp8 cache stores nodes otherwise than they are")
     scale = scale if scale is not None else 1.0 / math.sqrt(D)
@@ -121,9 +124,6 @@ def tree_attention(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         q, *kv = qkv[:, :(Hq + 2 * Hkv) * D].float().split([Hq * D, Hkv * D, Hkv * D], 1)
         qkv = torch.cat([q] + [kv_dequantize(*kv_quantize_rows(x.reshape(B * N, Hkv, D), k), k).view(B * N, Hkv * D) for x, k in zip(kv, (True, False))], 1)
     o = ref.tree_attention(qkv, k_cache, v_cache, kv_len, tree.see, Hq, kv_start, window, scale).to(kind)
-    key = _rows_of(Hkv, D, qkv.shape[1])
-    if key < 0:
-        raise ValueError(f"{Hkv} key heads of {D} in {qkv.shape[1]} columns")
     if tree.heads.setdefault(key, Hq) != Hq:
         tree.heads[key] = None
     return o if out is None else out.copy_(o)

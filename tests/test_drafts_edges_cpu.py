@@ -203,3 +203,16 @@ def test_accept_after_two_models_read_the_tree():
         ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]))
     ops.tree_accept(tree, tokens, tokens + 1, [a], kc, vc, _i32([0]), Hq=2)
     assert torch.equal(kc[0, 0, 0, :N], a[:, 2 * D:3 * D])
+
+
+def test_accept_of_rows_with_further_columns_read_as_stored():
+    B, N, Hq, Hkv, D, slots = 1, 3, 2, 1, 128, 9
+    rows = torch.randn(N, (Hq + 2 * Hkv) * D + D, generator=torch.Generator().manual_seed(0))
+    tree, tokens = ops.draft_tree(_i32([[-1, 0, 1]])), torch.arange(N)[None]
+    kc, vc = (torch.zeros(1, B, Hkv, slots, D, dtype=torch.uint8) for _ in "kv")
+    ks, vs = (torch.ones(1, B, Hkv, slots) for _ in "kv")
+    ops.tree_attention(rows, kc[0], vc[0], _i32([0]), tree, Hq, k_scale=ks[0], v_scale=vs[0], as_stored=True)
+    ops.tree_accept(tree, tokens, tokens + 1, [rows], kc, vc, _i32([0]), ks, vs)
+    for c, sc, at, key in ((kc, ks, Hq, True), (vc, vs, Hq + 1, False)):
+        q, s = ops.kv_quantize_rows(rows[:, at * D:(at + 1) * D], key)
+        assert torch.equal(c[0, 0, 0, :N], q) and torch.equal(sc[0, 0, 0, :N], s)
